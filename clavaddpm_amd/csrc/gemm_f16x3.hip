@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(64 * NW, OCC) gemm_f16x3_kernel(SplitGemmArgs 
     f32x2 ovf = {0.f, 0.f};
 
     // Per element the epilogue is VALU work (~13 instructions in the first straight-line version: 8.5 us of a 256 x 320
-    // tile's 7.4 + 1.5 us of prologue / epilogue at 160 elements per lane): it now runs on pairs of columns with the packed
-    // float32 instructions (v_pk_fma / v_pk_mul / v_pk_add) and v_cvt_pk_f16_f32, and, when only split rows go out and
+    // tile's 7.4 + 1.5 us of prologue / epilogue at 160 elements per lane): it now runs on pairs of columns with
+    // v_cvt_pk_f16_f32 (the float32 arithmetic itself is one element at a time: flags in build.py), and, when only split rows go out and
     // alpha == 1 (FOLD), with the output's power-of-two scale folded into the accumulator scale and the bias - exact, since
     // the activation is positively homogeneous and power-of-two factors commute with rounding: ~5 instructions per element.
     auto epilogue = [&](auto has_mask, auto out_mode, auto fold_t) {
