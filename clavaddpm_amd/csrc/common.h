@@ -39,6 +39,8 @@ enum ProfFamily {
     PROF_FUSED_NARROW = PROF_GEMM_F16X3 + PROF_GEMM_F16X3_CFGS,   // fused_narrow.hip
     PROF_GEMM_F16X3_TN,                                // gemm_f16x3_tn.hip
     PROF_CAT_INPUT,                                    // cat_input.hip
+    PROF_MX4,                                          // mx4.hip
+    PROF_CHOICE,                                       // choice.hip
     PROF_N_FAMILIES
 };
 extern bool g_clava_prof_on;

@@ -28,6 +28,11 @@ extern "C" {
 #define CLAVA_ACT_LEAKY_ 2 /* negative slope 0.01 = nn.LeakyReLU() default (pipeline_utils.py:615) */
 #define CLAVA_ACT_SILU_ 3
 
+/* element types of the entry points that take more than float32 */
+#define CLAVA_DT_F32 0
+#define CLAVA_DT_BF16 1
+#define CLAVA_DT_F16 2
+
 int clava_version(void);
 const char* clava_last_error(void);
 int clava_device_count(void); /* host-only probe: number of HIP devices, 0 when there is none */
@@ -138,6 +143,22 @@ int clava_gemm_wgrad_f16x3_tn(const void* dy, long long pitch_dy, int shift_dy, 
                               float* dw_slabs, int lddw, long long slab_stride, float* db_slabs, int M, int N_out, int K_in,
                               int splits, void* stream);
 
+/* ---- microscaled 4-bit matrices and dense layers over them (no counterpart in the reference) --------------------
+ * OCP microscaling (MX) with E2M1 elements (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives) and one E8M0 scale for every 32
+ * columns of a row.  With Kp = cols rounded up to 128:
+ *   codes  [rows][Kp / 2] bytes, column 2 i in the low and 2 i + 1 in the high four bits of byte i, zero behind the last column;
+ *   scales [rows][Kp / 32] bytes, value 2^(byte - 127), 255 = NaN.
+ * clava_mx4_pack: scale exponent e = floor(log2(max |v|)) - 2 (clamped to -127 .. 127), code = nearest E2M1 of v / 2^e, ties to
+ *   even, saturating at 6; a block that holds a NaN or an infinity gets scale 255 and reads as NaN.  src has row stride ld.
+ * clava_mx4_unpack: dst[r * ld + c] = value(code) * 2^(scale - 127), rounded to `dtype`.
+ * clava_linear_mx4: y[M,N] = act( x[M,K] . w[N,K]^T + bias[N] ), both operands as above, products summed in float32; the result
+ *   as `y` (y_dtype, row stride ldy) or, with y == NULL, packed again as y_codes / y_scales (for the next layer).  codes
+ *   pointers are 16-byte aligned.  dtype: CLAVA_DT_*; act: CLAVA_ACT_*_. */
+int clava_mx4_pack(const void* src, int dtype, long long ld, long long rows, int cols, void* codes, void* scales, void* stream);
+int clava_mx4_unpack(const void* codes, const void* scales, long long rows, int cols, void* dst, int dtype, long long ld, void* stream);
+int clava_linear_mx4(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, int act,
+                     void* y, int y_dtype, long long ldy, void* y_codes, void* y_scales, int M, int N, int K, void* stream);
+
 /* ---- schedule tables ---------------------------------------------------------------------------------------
  * Device-resident tables of length T, built by the host exactly as GaussianMultinomialDiffusion.__init__ builds
  * them (tab_ddpm/gaussian_multinomial_diffsuion.py:105-156); model_variance is the "fixed-large" variance the
@@ -206,6 +227,36 @@ int clava_multinomial_step_counter_f32(const clava_schedule* sched, int mode, in
  * previous setting; any other
  * `mode` only queries.  Process-wide; CLAVA_CAT_SAMPLER=gumbel|icdf sets the initial value. */
 int clava_categorical_sampler_set(int mode);
+
+/* One class per (row, feature) block from its logits, filtered (no counterpart in the reference, whose draws are unfiltered).
+ * Feature f of row b owns logits[b * ld + offsets[f] .. offsets[f+1]) (m features; offsets == NULL: one feature of sumK classes).
+ * With a_i = exp((z_i - max z) / temperature) and the classes ordered by falling z (equal ones by rising index):
+ *   top_k:  the first top_k of the order stay (<= 0 or >= the feature's classes: all);
+ *   top_p:  of those, the ones before which less than top_p of their mass lies (>= 1: all; the first always stays);
+ *   min_p:  of those, the ones with a_i >= min_p (the largest a is 1; values outside [0, 1] count as their nearest bound).
+ *   draw:   the first class, by index, up to which the kept mass exceeds u * (all kept mass).
+ * temperature 0 takes the first of the order.  A class with z = -inf is never drawn; where some z are +inf, those share the
+ * mass equally.  idx[b * m + f] = -1 (log_prob NaN) for a feature without classes, without a z above -inf, or with a NaN in
+ * its logits, its u or its temperature, or a negative temperature.  log_prob (optional) [B, m]: log of the drawn class's share of
+ * the kept mass.  Sums and comparisons are float64 and have a fixed order.
+ * Each parameter is a number for all blocks, or, where its pointer is not NULL, element [b * rs + f * fs] of a device array.
+ * uniforms [b * ld_u + f] in [0, 1), or NULL for the counter-based generator keyed by (seed, row_offset + b, f, step_index).
+ * max_k: the largest number of classes of one feature (a hint that picks the kernels; any value is safe).  workspace:
+ * clava_choice_workspace_bytes(B, m, max_k) bytes, 16-byte aligned (may be NULL where that is 0); its contents need not be kept. */
+typedef struct clava_choice {
+    double temperature, top_p, min_p;
+    int top_k;
+    const float* temperature_t;
+    const float* top_p_t;
+    const float* min_p_t;
+    const int* top_k_t;
+    long long temperature_rs, temperature_fs, top_p_rs, top_p_fs, min_p_rs, min_p_fs, top_k_rs, top_k_fs;
+} clava_choice;
+long long clava_choice_workspace_bytes(int B, int m, int max_k);
+int clava_sample_categories(const void* logits, int dtype, long long ld, int B, int m, int sumK, const int* offsets, int max_k,
+                            const clava_choice* choice, const float* uniforms, long long ld_u, unsigned long long seed,
+                            unsigned long long row_offset, unsigned step_index, int* idx, float* log_prob, void* workspace,
+                            long long workspace_bytes, void* stream);
 
 /* x_t[B,n_num] = sqrt_alphas_cumprod[t] * x0 + sqrt_one_minus_alphas_cumprod[t] * noise, per-row t (int64):
  * gaussian_q_sample (:172-180), float32. */
