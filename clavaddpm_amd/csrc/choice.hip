@@ -1,31 +1,44 @@
 // One class per (row, feature) block from its logits: temperature, top-k, top-p, min-p and the draw from a given uniform.
 //
-// The kept classes of top-k and top-p are a prefix of the order (z falling, index rising), so each is a threshold: all classes
-// with a key above t, and the first n of those with the key t.  Keys are float bits made monotone, so t is found bit by bit.
-// Masses a = exp((z - max) / T) are float64: a float32 running sum would put draws next to a border on its wrong side.
+// Masses a = exp((z - max) / T) are float64, or 64-bit integers counting 2^-s of the largest mass: a float32 running sum puts
+// draws next to a border on its wrong side, and integers add up to the same in every order.
+//
+// Top-k and top-p both keep a prefix of the order (z falling, index rising): the last kept class is the first one at which the
+// running weight (1 a class, or its mass) reaches a goal (k, or top_p of the mass).  So both are one search, "the edge":
+// classes fall into bins of falling z, the running weight over the bins names the bin of the edge, and only that bin's
+// classes are put in order.  Bins are linear in max - z (a logit's neighbours in z are its neighbours in mass too; bins of the
+// float's bits would put nearly all of them around z = 0), and where too many classes share one, its range of keys (float bits
+// made monotone) is cut again: six bits a time, down to equal keys, of which the first by index stay.
+//
+// Which kernel: up to 64 classes, a class a lane, in groups of 8 / 16 / 32 / 64 lanes; up to 64 * NV, a wavefront with the
+// block in LDS; wider ones are cut into chunks over many workgroups and joined (wide_*).
 #include "elem.h"
 #include "rng.h"
+#include "wave.h"
 
 namespace {
 using namespace elem;
+typedef unsigned long long u64;
 
 struct Choice {
     const void* z; long long ld;
     int B, m, sumK;
     const int* offsets;
     clava_choice p;
+    double c;                                 // log2(e) / temperature, where that is one number
     const float* u; long long ld_u;
     unsigned long long seed, row_offset;
     unsigned step;
     int* idx; float* log_prob;
+    int wide_from;                            // blocks with more classes belong to the wide_* kernels; 0: there are none
 };
 
-constexpr double LOG2E = 1.44269504088896340736;
+constexpr double LOG2E = 1.44269504088896340736, LN2 = 0.69314718055994530942;
 
-// 2^y for y <= 0: n = rint(y), 2^(y - n) by its power series (12 terms: ln2/2 ^ 13 / 13! < 2e-16), scaled by 2^n.
+// 2^y for y <= 0: n = rint(y), 2^(y - n) by its power series (12 terms: (ln2/2)^13 / 13! < 2e-16), scaled by 2^n.
 __device__ __forceinline__ double exp2_nonpos(double y) {
     y = fmax(y, -1100.0);                     // below float64's smallest subnormal
-    const double n = rint(y), r = (y - n) * 0.69314718055994530942;
+    const double n = rint(y), r = (y - n) * LN2;
     double p = 1.0 / 479001600;
     p = fma(p, r, 1.0 / 39916800);
     p = fma(p, r, 1.0 / 3628800);
@@ -41,176 +54,1085 @@ __device__ __forceinline__ double exp2_nonpos(double y) {
     p = fma(p, r, 1.0);
     return ldexp(p, (int)n);
 }
+// log(x) for x >= 1: the float32 logarithm and one Newton step on e^y = x (its square, 1e-14, is what stays)
+__device__ __forceinline__ double log_from1(double x) {
+    const double y = (double)logf((float)x);
+    return y + (x * exp2_nonpos(-y * LOG2E) - 1.0);
+}
 
 __device__ __forceinline__ unsigned key_of(float z) {
     const unsigned b = __float_as_uint(z + 0.f);              // -0 and +0 are one key
     return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
+// Position in the order: larger comes first; equal keys by index
+__device__ __forceinline__ u64 place_of(unsigned key, unsigned index) { return (u64)key << 32 | (unsigned)~index; }
 
-// Logits of a block relative to its maximum, as masses: +inf logits, where there are any, share the mass.
-struct Mass {
-    double top, c;                            // maximum, log2(e) / T
-    bool inf;
-    __device__ __forceinline__ double operator()(float z) const {
-        if (inf) return z == INFINITY ? 1.0 : 0.0;
-        return z == -INFINITY ? 0.0 : exp2_nonpos(((double)z - top) * c);
-    }
+// A block and its parameters, ready to use.
+struct Block {
+    int b, f, K;
+    size_t at;
+    double u, c, top_p, min_p;                // top_p in (0, 1], 1: off; min_p in [0, 1]
+    float T;                                  // for bin widths only
+    int top_k;                                // 0: off
+    bool bad;                                 // a parameter or u is not a number
 };
-
+__device__ __forceinline__ int first_of(const Choice& g, int f) { return g.offsets ? max(0, min(g.offsets[f], g.sumK)) : 0; }
+__device__ __forceinline__ int classes_of(const Choice& g, int f) {
+    return g.offsets ? max(0, min(g.offsets[f + 1], g.sumK) - first_of(g, f)) : g.sumK;
+}
 __device__ __forceinline__ double uniform_of(const Choice& g, int b, int f) {
     if (g.u) return (double)g.u[(size_t)b * g.ld_u + f];
     const unsigned long long e = (g.row_offset + (unsigned long long)b) * (unsigned long long)g.m + (unsigned long long)f;
     return (double)clava_rng::to_uniform(clava_rng::philox4x32_10(g.seed, e, g.step, clava_rng::STREAM_CHOICE).x);
 }
-
-constexpr int W = 256;
-
-template <class T> struct Sum { __device__ T operator()(T a, T b) const { return a + b; } };
-struct Max { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
-
-// Inclusive scan over the workgroup in thread order; s is W elements of LDS
-template <class T, class Op> __device__ __forceinline__ T scan(T v, T* s, Op op) {
-    const int t = threadIdx.x;
-    __syncthreads();
-    s[t] = v;
-    for (int d = 1; d < W; d *= 2) {
-        __syncthreads();
-        const T o = t >= d ? s[t - d] : v;
-        __syncthreads();
-        if (t >= d) { v = op(o, v); s[t] = v; }
+__device__ __forceinline__ Block block_of(const Choice& g, int b, int f, int k0, int K) {
+    Block x;
+    x.b = b; x.f = f; x.K = K;
+    x.at = (size_t)b * g.ld + k0;
+    x.u = uniform_of(g, b, f);
+    const clava_choice& p = g.p;
+    double T = p.temperature;
+    x.c = g.c;
+    if (p.temperature_t) {
+        T = (double)p.temperature_t[b * p.temperature_rs + f * p.temperature_fs];
+        x.c = LOG2E / T;
     }
-    __syncthreads();
+    x.top_p = p.top_p_t ? (double)p.top_p_t[b * p.top_p_rs + f * p.top_p_fs] : p.top_p;
+    x.min_p = p.min_p_t ? (double)p.min_p_t[b * p.min_p_rs + f * p.min_p_fs] : p.min_p;
+    x.top_k = p.top_k_t ? p.top_k_t[b * p.top_k_rs + f * p.top_k_fs] : p.top_k;
+    x.bad = x.u != x.u || !(T >= 0.0);
+    x.u = fmax(x.u, 0.0);
+    if (T < 1e-290) { x.c = LOG2E; T = 1.0; x.top_k = 1; }   // 0, and what 1 / T has no float64 for
+    x.T = (float)fmin(T, 1e30);
+    if (x.top_k < 0) x.top_k = 0;
+    x.min_p = fmin(fmax(x.min_p, 0.0), 1.0);                 // (fmax of a NaN: 0)
+    x.top_p = x.top_p < 1.0 ? fmax(x.top_p, 1e-290) : 1.0;   // the first of the order always stays; NaN: off
+    return x;
+}
+// log2 of a class's mass, and the mass; +inf logits, where there are any, share the mass
+__device__ __forceinline__ double log2_mass(float z, float top, double c) {
+    if (top == INFINITY) return z == INFINITY ? 0.0 : -INFINITY;
+    return z == -INFINITY ? -INFINITY : ((double)z - (double)top) * c;
+}
+__device__ __forceinline__ double mass_of(float z, float top, double c) { return exp2_nonpos(log2_mass(z, top, c)); }
+// a in units of 2^-s, s <= 51, to the nearest: the fraction bits of a * 2^s + 2^52
+__device__ __forceinline__ u64 units(double a, double scale) {
+    return (u64)__double_as_longlong(fma(a, scale, 0x1p52)) & 0xfffffffffffffull;
+}
+// The scale for K classes: their sum stays under 2^63, one mass under 2^52
+__device__ __forceinline__ double unit_scale(int K) {
+    const int s = min(51, 62 - (K > 1 ? 32 - (int)__builtin_clz((unsigned)(K - 1)) : 0));
+    return (double)(1ull << s);
+}
+// The goal of a draw among integer weights: the class up to which more than this is the one
+__device__ __forceinline__ u64 draw_goal(double u, u64 total) {
+    const double goal = u * (double)total;
+    return goal < (double)total ? min((u64)goal, total - 1) : total - 1;
+}
+
+__device__ __forceinline__ void give(const Choice& g, int b, int f, int idx, float lp) {
+    const size_t o = (size_t)b * g.m + f;
+    g.idx[o] = idx;
+    if (g.log_prob) g.log_prob[o] = lp;
+}
+__device__ __forceinline__ float no_number() { return __uint_as_float(0x7fc00000u); }
+
+// ------------------------------------------------------------------------------------------------------ lanes of a group
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ double dpp_d(double v) {      // 0 where there is no source lane
+    const u64 b = (u64)__double_as_longlong(v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+    return __longlong_as_double((long long)((u64)hi << 32 | lo));
+}
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ u64 dpp_d(u64 b) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+    return (u64)hi << 32 | lo;
+}
+// The lane, computed anew: what follows from it (a lane mask for every step of a sort) is not kept over a loop of blocks,
+// where it took 240 scalar registers
+__device__ __forceinline__ int lane_here() {
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    return l;
+}
+// Inclusive sums in lane order within groups of G lanes
+template <int G, class T> __device__ __forceinline__ T scan(T v) {
+    if (G == 8) {
+        const int l = lane_here();
+        T o = dpp_d<0x111>(v);
+        v += (l & 7) >= 1 ? o : T(0);
+        o = dpp_d<0x112>(v);
+        v += (l & 7) >= 2 ? o : T(0);
+        o = dpp_d<0x114>(v);
+        v += (l & 7) >= 4 ? o : T(0);
+        return v;
+    }
+    v += dpp_d<0x111>(v);                     // row_shr within rows of 16
+    v += dpp_d<0x112>(v);
+    v += dpp_d<0x114>(v);
+    v += dpp_d<0x118>(v);
+    if (G >= 32) v += dpp_d<0x142, 0xa>(v);   // the last lane of row 0 to row 1, of row 2 to row 3
+    if (G >= 64) v += dpp_d<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
     return v;
 }
-template <class T, class Op> __device__ __forceinline__ T reduce(T v, T* s, Op op) {
-    scan(v, s, op);
-    return s[W - 1];
+__device__ __forceinline__ u64 from_lane(u64 v, int lane) {
+    return (u64)(unsigned)__shfl((int)(v >> 32), lane, 64) << 32 | (unsigned)__shfl((int)v, lane, 64);
+}
+__device__ __forceinline__ double from_lane(double v, int lane) {
+    return __longlong_as_double((long long)from_lane((u64)__double_as_longlong(v), lane));
+}
+__device__ __forceinline__ u64 from_xor(u64 v, int mask) {
+    return (u64)(unsigned)__shfl_xor((int)(v >> 32), mask, 64) << 32 | (unsigned)__shfl_xor((int)v, mask, 64);
+}
+// Bitonic sort within groups of G lanes, largest first
+template <int G> __device__ __forceinline__ u64 sort_falling(u64 v) {
+    const int l = lane_here() & (G - 1);
+#pragma unroll
+    for (int k = 2; k <= G; k *= 2)
+#pragma unroll
+        for (int d = k / 2; d > 0; d /= 2) {
+            const u64 o = from_xor(v, d);
+            const bool larger = ((l & d) == 0) == ((l & k) == 0 || k == G);
+            v = (v > o) == larger ? v : o;
+        }
+    return v;
 }
 
-template <int DT> __global__ void __launch_bounds__(W) choose_kernel(Choice g) {
-    __shared__ double sd[W];
-    __shared__ float sf[W];
-    __shared__ int si[W];
-    const int t = threadIdx.x;
-    for (long long blk = blockIdx.x; blk < (long long)g.B * g.m; blk += gridDim.x) {
-        const int b = (int)(blk / g.m), f = (int)(blk - (long long)b * g.m);
-        const int k0 = g.offsets ? max(0, min(g.offsets[f], g.sumK)) : 0;
-        const int K = (g.offsets ? max(k0, min(g.offsets[f + 1], g.sumK)) : g.sumK) - k0;
-        const size_t at = (size_t)b * g.ld + k0;
-        const double u = uniform_of(g, b, f);
-        const clava_choice& p = g.p;
-        double T = p.temperature_t ? (double)p.temperature_t[b * p.temperature_rs + f * p.temperature_fs] : p.temperature;
-        double top_p = p.top_p_t ? (double)p.top_p_t[b * p.top_p_rs + f * p.top_p_fs] : p.top_p;
-        double min_p = p.min_p_t ? (double)p.min_p_t[b * p.min_p_rs + f * p.min_p_fs] : p.min_p;
-        int top_k = p.top_k_t ? p.top_k_t[b * p.top_k_rs + f * p.top_k_fs] : p.top_k;
-        float mx = -INFINITY;
-        int nan = 0;
-        for (int i = t; i < K; i += W) {
-            const float z = load1<DT>(g.z, at + i);
-            nan |= z != z;
-            mx = fmaxf(mx, z);
-        }
-        mx = reduce(mx, sf, Max());
-        nan = reduce(nan, si, Sum<int>());
-        if (nan || mx == -INFINITY || u != u || !(T >= 0.0)) {
-            if (t == 0) {
-                g.idx[blk] = -1;
-                if (g.log_prob) g.log_prob[blk] = __uint_as_float(0x7fc00000u);
+// The whole choice among the classes that a group's lanes hold, one each, in index order: `z` (-inf and key 0 where a lane holds
+// none), their index, the block's maximum.  `nan`: the block holds a NaN.  All lanes of the wave come here together.
+template <int G> __device__ __forceinline__ void choose_lanes(const Choice& g, const Block& x, float z, unsigned key, int index, float top,
+                                                              bool nan, bool live) {
+    const int lane = threadIdx.x & 63, base = lane & ~(G - 1), l = lane & (G - 1);
+    const u64 group = (G == 64 ? ~0ull : ((1ull << G) - 1)) << base;
+    const double y = log2_mass(z, top, x.c), a = exp2_nonpos(y);
+    bool keep = a >= x.min_p;
+    if (__any(x.top_k > 0 || x.top_p < 1.0)) {
+        const u64 place = (u64)key << 32 | (unsigned)(63 - lane);
+        const u64 sorted = sort_falling<G>(place);
+        const bool in = x.top_k == 0 || l < x.top_k;
+        const double as = from_lane(a, 63 - (int)(unsigned)sorted);
+        const double w = in ? as : 0.0, run = scan<G>(w);
+        const double goal = x.top_p * from_lane(run, base + G - 1);
+        const bool stay = in && (l == 0 || x.top_p >= 1.0 || run - w < goal);
+        const u64 out = ~(__ballot(stay) >> base) | (G == 64 ? 0 : 1ull << (G & 63));
+        const int n = out ? (int)__builtin_ctzll(out) : 64;      // those before the first that goes
+        const u64 last = from_lane(sorted, base + n - 1);        // (every lane gives its own: not behind a lane's condition)
+        keep = keep && place >= last;
+    }
+    const double w = keep ? a : 0.0, run = scan<G>(w), total = from_lane(run, base + G - 1);
+    const double goal = x.u * total;
+    const u64 can = __ballot(w > 0.0) & group, past = __ballot(w > 0.0 && run > goal) & group;
+    if (!live) return;
+    const bool none = nan || x.bad || top == -INFINITY;
+    const int hit = past ? (int)__builtin_ctzll(past) : can ? 63 - (int)__builtin_clzll(can) : 0;
+    if (none ? l == 0 : lane == hit) give(g, x.b, x.f, none ? -1 : index, none ? no_number() : (float)(y * LN2 - log_from1(total)));
+}
+
+// ---------------------------------------------------------------------------------------------------- a wavefront's block
+// What a wavefront keeps in LDS beside its block's logits: bins, then the classes of one bin
+struct WaveLds {
+    u64 bin[64];
+    u64 place[64];
+    u64 weight[64];
+};
+// Bins per unit of max - z: over the range of the logits, or 40 T where that is less (no mass is left beyond it, and what
+// shares the last bin is cut again if an edge falls into it).  0: all classes share the first bin, for ranges that are not
+// numbers or have no inverse.
+__device__ __forceinline__ float bins_per_unit(float top, float bottom, float T, float bins) {
+    const float range = fminf(top - bottom, 40.f * T), inv = bins / range;
+    return top < INFINITY && range > 0.f && range < 1e37f && inv < 1e37f ? inv : 0.f;
+}
+__device__ __forceinline__ int linear_bin(float z, float top, float inv, int bins) {
+    return inv > 0.f ? (int)fminf((top - z) * inv, (float)(bins - 1)) : 0;
+}
+// LDS of one wavefront is read and written in program order; this keeps the compiler to it
+__device__ __forceinline__ void lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ unsigned wave_min(unsigned v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = min(v, (unsigned)__shfl_xor((int)v, o, 64));
+    return v;
+}
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+    return v;
+}
+
+// The block's classes by slots of 64: logit `z[j * 64 + lane]` in LDS, -inf behind the last one
+struct WaveBlock {
+    const float* z;
+    int n;                                                   // slots
+    float top, inv;
+};
+// Weights in 64 linear bins of falling z (lane l: bin l)
+template <class In, class Weight> __device__ __forceinline__ u64 bins_of(const WaveBlock& w, WaveLds& s, In in, Weight weight) {
+    const int lane = threadIdx.x & 63;
+    s.bin[lane] = 0;
+    lds_order();
+    for (int j = 0; j < w.n; ++j) {
+        const float z = w.z[j * 64 + lane];
+        if (in(z, j)) atomicAdd(&s.bin[linear_bin(z, w.top, w.inv, 64)], weight(z));
+    }
+    lds_order();
+    return s.bin[lane];
+}
+// The place of the first class, in falling order, at which the running weight reaches `goal`; 0 if none does.  The classes are
+// those with in(z, slot), `bins` their weights by bins_of.
+template <class In, class Weight>
+__device__ __forceinline__ u64 find_edge(const WaveBlock& w, u64 bins, double goal, WaveLds& s, In in, Weight weight) {
+    const int lane = threadIdx.x & 63;
+    unsigned lo = 0, hi = 0xffffffffu;                       // keys of the classes that are left
+    u64 before = 0;
+    int shift = -1;                                          // < 0: linear bins
+    for (;;) {
+        const u64 run = scan<64>(bins), past = __ballot((double)(before + run) >= goal);
+        if (past == 0) return 0;
+        const int at = (int)__builtin_ctzll(past);
+        before += from_lane(run - bins, at);
+        // the classes of that bin
+        int count = 0;
+        unsigned klo = 0xffffffffu, khi = 0;
+        for (int j = 0; j < w.n; ++j) {
+            const float z = w.z[j * 64 + lane];
+            const unsigned key = key_of(z);
+            const bool is = in(z, j) && key >= lo && key <= hi &&
+                            (shift < 0 ? linear_bin(z, w.top, w.inv, 64) : (int)((hi - key) >> shift)) == at;
+            const u64 who = __ballot(is);
+            if (who == 0) continue;
+            const int pos = count + (int)__popcll(who & ((1ull << lane) - 1));
+            if (is) {
+                if (pos < 64) { s.place[pos] = place_of(key, (unsigned)(j * 64 + lane)); s.weight[pos] = weight(z); }
+                klo = min(klo, key);
+                khi = max(khi, key);
             }
-            continue;
+            count += (int)__popcll(who);
         }
-        if (T < 1e-290) { T = 1.0; top_k = 1; }           // 0, and what 1 / T has no float64 for
-        min_p = fmin(fmax(min_p, 0.0), 1.0);              // (fmax of a NaN: 0)
-        top_p = fmax(top_p, 1e-290);                      // the first of the order always stays
-        const Mass mass{(double)mx, LOG2E / T, mx == INFINITY};
-        // keep: key above `edge`, or the first `ties` with that key
-        unsigned edge = 0;
-        int ties = K;
-        const bool cut_k = top_k > 0 && top_k < K, cut_p = top_p < 1.0;
-        if (cut_k) {
-            for (int bit = 31; bit >= 0; --bit) {
-                const unsigned at_least = edge | 1u << bit;
-                int n = 0;
-                for (int i = t; i < K; i += W) n += key_of(load1<DT>(g.z, at + i)) >= at_least;
-                if (reduce(n, si, Sum<int>()) >= top_k) edge = at_least;
-            }
-            int above = 0;
-            for (int i = t; i < K; i += W) above += key_of(load1<DT>(g.z, at + i)) > edge;
-            ties = top_k - reduce(above, si, Sum<int>());
+        lds_order();
+        if (count <= 64) {
+            const u64 mine = lane < count ? s.place[lane] : 0;
+            // sorted with the position in the list, which is in index order, instead of the index
+            const u64 sorted = sort_falling<64>(lane < count ? (mine >> 32 << 32 | (unsigned)(63 - lane)) : 0);
+            const int pos = 63 - (int)(sorted & 63);
+            const u64 sum = scan<64>(lane < count ? s.weight[pos] : (u64)0);
+            const u64 there = __ballot(lane < count && (double)(before + sum) >= goal);
+            return from_lane(mine, __shfl(pos, there ? (int)__builtin_ctzll(there) : count - 1, 64));
         }
-        if (cut_p) {
-            // mass of the keys >= `least` that top-k left
-            auto mass_from = [&](unsigned least) {
-                double s = 0.0;
-                for (int i = t; i < K; i += W) {
-                    const float z = load1<DT>(g.z, at + i);
-                    const unsigned k = key_of(z);
-                    if (k >= least && (!cut_k || k > edge)) s += mass(z);
+        lo = wave_min(klo);
+        hi = wave_max(khi);
+        if (lo == hi) {                                      // equal keys, equal weights: the first so many by index
+            const double one = (double)s.weight[0], need = one > 0.0 ? ceil((goal - (double)before) / one) : (double)count;
+            int left = max(1, (int)fmin(fmax(need, 1.0), (double)count));
+            for (int j = 0; j < w.n; ++j) {
+                const float z = w.z[j * 64 + lane];
+                u64 who = __ballot(in(z, j) && key_of(z) == lo);
+                const int c = (int)__popcll(who);
+                if (left <= c) {
+                    for (int k = 1; k < left; ++k) who &= who - 1;
+                    return place_of(lo, (unsigned)(j * 64 + (int)__builtin_ctzll(who)));
                 }
-                return reduce(s, sd, Sum<double>());
-            };
-            const float edge_z = __uint_as_float(edge & 0x80000000u ? edge ^ 0x80000000u : ~edge);
-            const double at_edge = cut_k ? ties * mass(edge_z) : 0.0;
-            const double goal = top_p * (mass_from(0) + at_edge);
-            unsigned e = 0;
-            for (int bit = 31; bit >= 0; --bit) {
-                const unsigned least = e | 1u << bit;
-                if (mass_from(least) + (cut_k && least <= edge ? at_edge : 0.0) >= goal) e = least;
+                left -= c;
             }
-            // e: the key at which the prefix reaches the goal; how many of that key
-            if (!cut_k || e > edge) {
-                int n = 0;
-                for (int i = t; i < K; i += W) n += key_of(load1<DT>(g.z, at + i)) == e;
-                ties = reduce(n, si, Sum<int>());
-            }
-            const double before = e == 0xffffffffu ? 0.0 : mass_from(e + 1);
-            edge = e;
-            const double one = mass(__uint_as_float(e & 0x80000000u ? e ^ 0x80000000u : ~e));
-            const double n = one > 0.0 ? ceil((goal - before) / one) : (double)ties;
-            ties = max(1, (int)fmin(fmax(n, 1.0), (double)ties));
         }
-        // the draw: a run of neighbouring classes a thread, so that sums follow the index
-        const int per = (K + W - 1) / W, i0 = min(K, t * per), i1 = min(K, i0 + per);
-        int eq = 0;
-        for (int i = i0; i < i1; ++i) eq += key_of(load1<DT>(g.z, at + i)) == edge;
-        int seen = scan(eq, si, Sum<int>()) - eq;
-        const int seen0 = seen;
-        auto kept = [&](float z) {
-            const unsigned k = key_of(z);
-            const bool in = k > edge || (k == edge && seen < ties);
-            seen += k == edge;
-            const double a = in ? mass(z) : 0.0;
-            return a >= min_p ? a : 0.0;
-        };
-        double own = 0.0;
-        for (int i = i0; i < i1; ++i) own += kept(load1<DT>(g.z, at + i));
-        scan(own, sd, Sum<double>());
-        const double total = sd[W - 1], goal = fmin(fmax(u, 0.0) * total, total * (1.0 - 0x1p-50));
-        double run = t ? sd[t - 1] : 0.0;
-        if (run <= goal && sd[t] > goal) {
-            seen = seen0;
-            int hit = -1;
-            double a_hit = 0.0;
-            for (int i = i0; i < i1; ++i) {
-                const double a = kept(load1<DT>(g.z, at + i));
-                run += a;
-                if (a > 0.0) {
-                    hit = i;
-                    a_hit = a;
-                    if (run > goal) break;
-                }
+        shift = max(0, 26 - (int)__builtin_clz(hi - lo));    // (hi - lo) >> shift < 64
+        lds_order();
+        s.bin[lane] = 0;
+        lds_order();
+        for (int j = 0; j < w.n; ++j) {
+            const float z = w.z[j * 64 + lane];
+            const unsigned key = key_of(z);
+            if (in(z, j) && key >= lo && key <= hi) atomicAdd(&s.bin[(hi - key) >> shift], weight(z));
+        }
+        lds_order();
+        bins = s.bin[lane];
+    }
+}
+
+// Sums over the wave of four values at once: halves, then rows of 16 change places, so that row r ends up with value r
+__device__ __forceinline__ void swap32(double& a, double& b) {
+    const u64 p = (u64)__double_as_longlong(a), q = (u64)__double_as_longlong(b);
+    const auto lo = __builtin_amdgcn_permlane32_swap((unsigned)p, (unsigned)q, false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap((unsigned)(p >> 32), (unsigned)(q >> 32), false, false);
+    a = __longlong_as_double((long long)((u64)hi[0] << 32 | lo[0]));
+    b = __longlong_as_double((long long)((u64)hi[1] << 32 | lo[1]));
+}
+__device__ __forceinline__ void swap16(double& a, double& b) {
+    const u64 p = (u64)__double_as_longlong(a), q = (u64)__double_as_longlong(b);
+    const auto lo = __builtin_amdgcn_permlane16_swap((unsigned)p, (unsigned)q, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((unsigned)(p >> 32), (unsigned)(q >> 32), false, false);
+    a = __longlong_as_double((long long)((u64)hi[0] << 32 | lo[0]));
+    b = __longlong_as_double((long long)((u64)hi[1] << 32 | lo[1]));
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+    const u64 b = (u64)__double_as_longlong(v);
+    return __longlong_as_double((long long)((u64)(unsigned)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 |
+                                            (unsigned)__builtin_amdgcn_readlane((int)b, lane)));
+}
+__device__ __forceinline__ void sums4(double (&v)[4]) {
+    swap32(v[0], v[2]);
+    swap32(v[1], v[3]);
+    double a = v[0] + v[2], b = v[1] + v[3];
+    swap16(a, b);
+    a += b;
+    a += dpp_d<DPP_XOR1>(a);
+    a += dpp_d<DPP_XOR2>(a);
+    a += dpp_d<DPP_HALF_MIRROR>(a);
+    a += dpp_d<DPP_ROW_MIRROR>(a);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = lane_value(a, 16 * r);
+}
+
+// A block of up to 64 * (floats of zs / 64) classes.  Its logits stay in LDS: the passes over them are loops of a run-time
+// length then, and the compiler keeps no register per slot (with the block in registers the unrolled passes took 232 of them
+// and two wavefronts a SIMD).
+template <int DT> __device__ __forceinline__ void choose_wave(const Choice& g, const Block& x, float* zs, WaveLds& s) {
+    const int lane = threadIdx.x & 63;
+    WaveBlock w;
+    w.z = zs;
+    w.n = (x.K + 63) >> 6;
+    float top = -INFINITY, bottom = INFINITY;
+    bool nan = false;
+    lds_order();
+#pragma unroll 4
+    for (int j = 0; j < w.n; ++j) {
+        const int i = j * 64 + lane;
+        const float z = i < x.K ? load1<DT>(g.z, x.at + i) : -INFINITY;
+        nan |= z != z;
+        top = fmaxf(top, z);
+        bottom = z == -INFINITY ? bottom : fminf(bottom, z);
+        zs[i] = z;
+    }
+    lds_order();
+    top = group_max<64>(top);
+    if (__any(nan) || x.bad || top == -INFINITY) {
+        if (lane == 0) give(g, x.b, x.f, -1, no_number());
+        return;
+    }
+    const bool cut_k = x.top_k > 0 && x.top_k < x.K, cut_p = x.top_p < 1.0;
+    w.top = top;
+    w.inv = cut_k || cut_p ? bins_per_unit(top, -group_max<64>(-bottom), x.T, 64.f) : 0.f;
+    u64 edge = 0;
+    if (cut_k) {
+        auto in = [](float z, int) { return z > -INFINITY; };                    // (-inf: no mass, behind every other class)
+        auto one = [](float) { return (u64)1; };
+        const u64 bins = bins_of(w, s, in, one);
+        const u64 run = scan<64>(bins), past = __ballot((int)run >= x.top_k);
+        const int at = past ? (int)__builtin_ctzll(past) : 63, n = (int)from_lane(run, at);
+        if (n <= 64) {
+            // few enough for a class a lane: everything else is done there
+            int count = 0;
+            float zl = -INFINITY;
+            lds_order();
+            for (int j = 0; j < w.n; ++j) {
+                const float z = zs[j * 64 + lane];
+                const bool is = z > -INFINITY && linear_bin(z, top, w.inv, 64) <= at;
+                const u64 who = __ballot(is);
+                const int pos = count + (int)__popcll(who & ((1ull << lane) - 1));
+                if (is) s.place[pos] = (u64)__float_as_uint(z) << 32 | (unsigned)(j * 64 + lane);
+                count += (int)__popcll(who);
             }
-            g.idx[blk] = hit;
-            if (g.log_prob) g.log_prob[blk] = (float)log(a_hit / total);
+            lds_order();
+            const u64 mine = s.place[lane];
+            if (lane < n) zl = __uint_as_float((unsigned)(mine >> 32));
+            choose_lanes<64>(g, x, zl, lane < n ? key_of(zl) : 0u, (int)(unsigned)mine, top, false, true);
+            return;
+        }
+        edge = find_edge(w, bins, (double)x.top_k, s, in, one);
+    }
+    auto stays = [&](float z, int j) { return edge == 0 || place_of(key_of(z), (unsigned)(j * 64 + lane)) >= edge; };
+    if (cut_p) {
+        const double scale = unit_scale(2048);
+        auto in = [&](float z, int j) { return z > -INFINITY && stays(z, j); };
+        auto weight = [&](float z) { return units(mass_of(z, top, x.c), scale); };
+        const u64 bins = bins_of(w, s, in, weight);
+        const u64 to = find_edge(w, bins, x.top_p * (double)from_lane(scan<64>(bins), 63), s, in, weight);
+        edge = max(edge, to);
+    }
+    auto mass = [&](int j) {
+        const float z = zs[j * 64 + lane];
+        const double a = mass_of(z, top, x.c);
+        return stays(z, j) && a >= x.min_p ? a : 0.0;
+    };
+    // where the running mass passes the goal: in which quarter of the slots, then of that quarter's, down to one slot
+    double before = 0.0, goal = 0.0, total = 0.0;
+    int from = 0, to = w.n;
+    for (bool first = true;; first = false) {
+        const int q = (to - from + 3) >> 2;
+        double v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            v[r] = 0.0;
+            for (int j = from + r * q; j < min(to, from + (r + 1) * q); ++j) v[r] += mass(j);
+        }
+        sums4(v);
+        if (first) {
+            total = v[0] + v[1] + v[2] + v[3];
+            goal = fmin(x.u * total, total * (1.0 - 0x1p-50));
+        }
+        int pick = 0;
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (pick == k && before + v[k] <= goal && from + (k + 1) * q < to) { before += v[k]; ++pick; }
+        from += pick * q;
+        to = min(to, from + q);
+        if (q == 1) break;
+    }
+    const double mine = mass(from), run = before + scan<64>(mine);
+    const u64 can = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && run > goal);
+    int hit = past ? (int)__builtin_ctzll(past) : can ? 63 - (int)__builtin_clzll(can) : -1;
+    for (int j = w.n; hit < 0 && --j >= 0;) {   // rounding led to a slot without mass: the last class that has some
+        const u64 who = __ballot(mass(j) > 0.0);
+        if (who) { hit = 63 - (int)__builtin_clzll(who); from = j; }
+    }
+    if (lane == hit) give(g, x.b, x.f, from * 64 + lane, (float)(log2_mass(zs[from * 64 + lane], top, x.c) * LN2 - log_from1(total)));
+}
+
+// --------------------------------------------------------------------------------------- any block, any number of classes
+// A team of TH threads (a wavefront, or a workgroup) over data that it reads again in every pass: the edge byte by byte of
+// the place.  Behind wide blocks whose bins hold too many classes, and for blocks wider than `max_k` said.
+struct TeamLds {
+    u64 weight[256];
+    unsigned count[256];
+    u64 part[8];
+    u64 out[3];
+};
+template <int TH> __device__ __forceinline__ void team_sync() {
+    if (TH == 64) lds_order();
+    else __syncthreads();
+}
+// Inclusive sums in thread order; `total` gets the last
+template <int TH> __device__ __forceinline__ u64 team_scan(u64 v, TeamLds& s, u64& total) {
+    u64 run = scan<64>(v);
+    if (TH == 64) {
+        total = from_lane(run, 63);
+        return run;
+    }
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) s.part[wave] = run;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < TH / 64; ++w) {
+        if (w < wave) run += s.part[w];
+        total += s.part[w];
+    }
+    return run;
+}
+// The place of the first class in order at which `before` + the running weight reaches `goal`; 0 if none does.
+// each(f): f(place, weight) for all classes, split over the team.
+template <int TH, class Each> __device__ __forceinline__ u64 team_edge(double goal, u64 before, TeamLds& s, Each each) {
+    const int t = TH == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
+    u64 prefix = 0, mask = 0;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        team_sync<TH>();
+        for (int i = t; i < 256; i += TH) { s.weight[i] = 0; s.count[i] = 0; }
+        team_sync<TH>();
+        each([&](u64 place, u64 w) {
+            if ((place & mask) == prefix) {
+                const int bin = 255 - (int)(place >> shift & 255);
+                atomicAdd(&s.weight[bin], w);
+                atomicAdd(&s.count[bin], 1u);
+            }
+        });
+        team_sync<TH>();
+        if (t < 64) {
+            u64 own[4], sum = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { own[k] = s.weight[4 * t + k]; sum += own[k]; }
+            const u64 run = scan<64>(sum);
+            const u64 past = __ballot((double)(before + run) >= goal);
+            if (past == 0) {
+                if (t == 0) s.out[0] = 256;
+            } else if (t == (int)__builtin_ctzll(past)) {
+                u64 b = before + run - sum;
+                int k = 0;
+                while (k < 3 && (double)(b + own[k]) < goal) b += own[k++];
+                s.out[0] = (u64)(4 * t + k);
+                s.out[1] = b;
+            }
+        }
+        team_sync<TH>();
+        if (s.out[0] == 256) return 0;
+        before = s.out[1];
+        prefix |= (u64)(255 - s.out[0]) << shift;
+        mask |= 255ull << shift;
+        if (s.count[s.out[0]] == 1 && shift) {
+            each([&](u64 place, u64) {
+                if ((place & mask) == prefix) s.out[2] = place;
+            });
+            team_sync<TH>();
+            return s.out[2];
         }
     }
+    return prefix;
+}
+// The draw among classes i0 .. i1 of a block, as weights in index order: the first at which `before` + the running weight
+// passes `goal` (u == 0: the first with any mass, also one that is under half a unit).  `total`: the kept mass in units.
+template <int TH, int DT>
+__device__ __forceinline__ void team_draw(const Choice& g, const Block& x, float top, u64 edge, double scale, int i0, int i1, u64 before,
+                                          u64 goal, u64 total, TeamLds& s) {
+    const int t = TH == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
+    const int per = (i1 - i0 + TH - 1) / TH, from = min(i1, i0 + t * per), to = min(i1, from + per);
+    auto weight = [&](int i, float z, bool& any) {
+        const double a = place_of(key_of(z), (unsigned)i) >= edge ? mass_of(z, top, x.c) : 0.0;
+        any = a > 0.0 && a >= x.min_p;
+        return any ? x.u == 0.0 ? (u64)1 : units(a, scale) : (u64)0;
+    };
+    u64 own = 0, all;
+    bool any;
+    for (int i = from; i < to; ++i) own += weight(i, load1<DT>(g.z, x.at + i), any);
+    if (x.u == 0.0) { before = 0; goal = 0; }
+    u64 run = before + team_scan<TH>(own, s, all) - own;
+    if (own && run <= goal && run + own > goal) {
+        int hit = from;
+        for (int i = from; i < to; ++i) {
+            const u64 w = weight(i, load1<DT>(g.z, x.at + i), any);
+            run += w;
+            if (w) hit = i;
+            if (w && run > goal) break;
+        }
+        const double y = log2_mass(load1<DT>(g.z, x.at + hit), top, x.c);
+        give(g, x.b, x.f, hit, (float)(y * LN2 - log_from1((double)total / scale)));
+    }
+}
+template <int TH, int DT> __device__ void choose_team(const Choice& g, const Block& x, TeamLds& s) {
+    const int t = TH == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
+    float top = -INFINITY;
+    u64 bad = 0;
+    for (int i = t; i < x.K; i += TH) {
+        const float z = load1<DT>(g.z, x.at + i);
+        bad += z != z;
+        top = fmaxf(top, z);
+    }
+    u64 nan;
+    team_scan<TH>(bad, s, nan);
+    team_sync<TH>();
+    top = group_max<64>(top);
+    if (TH > 64) {
+        if ((t & 63) == 0) s.part[t >> 6] = __float_as_uint(top);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < TH / 64; ++w) top = fmaxf(top, __uint_as_float((unsigned)s.part[w]));
+        __syncthreads();
+    }
+    if (nan || x.bad || top == -INFINITY) {
+        if (t == 0) give(g, x.b, x.f, -1, no_number());
+        return;
+    }
+    const double scale = unit_scale(x.K);
+    u64 edge = 0;
+    if (x.top_k > 0 && x.top_k < x.K)
+        edge = team_edge<TH>((double)x.top_k, 0, s, [&](auto f) {
+            for (int i = t; i < x.K; i += TH) {
+                const float z = load1<DT>(g.z, x.at + i);
+                if (z > -INFINITY) f(place_of(key_of(z), (unsigned)i), 1);
+            }
+        });
+    u64 sum = 0, total;
+    for (int i = t; i < x.K; i += TH) {
+        const float z = load1<DT>(g.z, x.at + i);
+        if (place_of(key_of(z), (unsigned)i) >= edge) sum += units(mass_of(z, top, x.c), scale);
+    }
+    team_scan<TH>(sum, s, total);
+    if (x.top_p < 1.0) {
+        const u64 to = team_edge<TH>(x.top_p * (double)total, 0, s, [&](auto f) {
+            for (int i = t; i < x.K; i += TH) {
+                const float z = load1<DT>(g.z, x.at + i);
+                const u64 place = place_of(key_of(z), (unsigned)i);
+                if (place >= edge) f(place, units(mass_of(z, top, x.c), scale));
+            }
+        });
+        edge = max(edge, to);
+    }
+    if (x.top_p < 1.0 || x.min_p > 0.0) {
+        sum = 0;
+        for (int i = t; i < x.K; i += TH) {
+            const float z = load1<DT>(g.z, x.at + i);
+            const double a = place_of(key_of(z), (unsigned)i) >= edge ? mass_of(z, top, x.c) : 0.0;
+            if (a >= x.min_p) sum += units(a, scale);
+        }
+        team_scan<TH>(sum, s, total);
+    }
+    team_draw<TH, DT>(g, x, top, edge, scale, 0, x.K, 0, draw_goal(x.u, total), total, s);
+}
+
+// ----------------------------------------------------------------------------------- rows of features, block by block
+constexpr int WAVES = 4;
+template <int NV> union WaveMemory {
+    struct {
+        WaveLds lds;
+        float z[NV * 64];
+    } wave;
+    TeamLds team;
+};
+
+// Blocks of at most G classes, 64 / G of one row at a time; a wavefront takes a run of neighbouring items
+template <int DT, int G>
+__device__ __forceinline__ void choose_narrow(const Choice& g, const int* perm, const int* off, int n, unsigned wave, unsigned waves) {
+    if (n == 0) return;
+    constexpr unsigned PER = 64 / G;
+    const int lane = threadIdx.x & 63, l = lane & (G - 1);
+    const unsigned per_row = ((unsigned)n + PER - 1) / PER, items = per_row * (unsigned)g.B;
+    const unsigned i0 = (unsigned)((u64)items * wave / waves), i1 = (unsigned)((u64)items * (wave + 1) / waves);
+    unsigned b = i0 / per_row, w = i0 - b * per_row;
+    for (unsigned it = i0; it < i1; ++it) {
+        const int slot = (int)(w * PER) + lane / G;
+        const bool live = slot < n;
+        const int f = perm[live ? slot : n - 1], k0 = off[f], K = max(0, off[f + 1] - k0);
+        const Block x = block_of(g, (int)b, f, k0, K);
+        const float z = l < K ? load1<DT>(g.z, x.at + l) : -INFINITY;
+        const u64 group = ((G == 64 ? 0ull : 1ull << (G & 63)) - 1) << (lane & ~(G - 1));
+        const bool nan = (__ballot(z != z) & group) != 0;
+        choose_lanes<G>(g, x, z, l < K ? key_of(z) : 0u, l, group_max<G>(z), nan, live);
+        if (++w == per_row) { w = 0; ++b; }
+    }
+}
+
+template <int DT, int NV> __global__ void __launch_bounds__(WAVES * 64) choose_kernel(Choice g) {
+    __shared__ int s_off[MAX_LDS_FEATURES + 1], s_perm[MAX_LDS_FEATURES], s_start[5];
+    __shared__ WaveMemory<NV> s_mem[WAVES];
+    const bool order = g.m <= MAX_LDS_FEATURES;
+    if (order) {
+        for (int i = threadIdx.x; i <= g.m; i += WAVES * 64)
+            s_off[i] = g.offsets ? max(0, min(g.offsets[i], g.sumK)) : i ? g.sumK : 0;
+        __syncthreads();
+        order_features_by_width(g.m, s_off, s_perm, s_start);
+    }
+    const unsigned wave = blockIdx.x * WAVES + (threadIdx.x >> 6), waves = gridDim.x * WAVES;
+    WaveMemory<NV>& mem = s_mem[threadIdx.x >> 6];
+    if (order) {
+        choose_narrow<DT, 8>(g, s_perm, s_off, s_start[1], wave, waves);
+        choose_narrow<DT, 16>(g, s_perm + s_start[1], s_off, s_start[2] - s_start[1], wave, waves);
+        choose_narrow<DT, 32>(g, s_perm + s_start[2], s_off, s_start[3] - s_start[2], wave, waves);
+    }
+    const unsigned first = order ? (unsigned)s_start[3] : 0u, n = (unsigned)g.m - first;
+    if (n == 0) return;
+    const unsigned items = n * (unsigned)g.B;
+    const unsigned i0 = (unsigned)((u64)items * wave / waves), i1 = (unsigned)((u64)items * (wave + 1) / waves);
+    unsigned b = i0 / n, w = i0 - b * n;
+    const int lane = threadIdx.x & 63;
+    for (unsigned it = i0; it < i1; ++it) {
+        const int f = __builtin_amdgcn_readfirstlane(order ? s_perm[first + w] : (int)w);
+        const int k0 = __builtin_amdgcn_readfirstlane(order ? s_off[f] : first_of(g, f));
+        const int K = __builtin_amdgcn_readfirstlane(order ? max(0, s_off[f + 1] - k0) : classes_of(g, f));
+        if (!g.wide_from || K <= g.wide_from) {
+            const Block x = block_of(g, (int)b, f, k0, K);
+            if (K <= 64) {
+                const float z = lane < K ? load1<DT>(g.z, x.at + lane) : -INFINITY;
+                choose_lanes<64>(g, x, z, lane < K ? key_of(z) : 0u, lane, group_max<64>(z), __any(z != z), true);
+            } else if (K <= NV * 64) {
+                choose_wave<DT>(g, x, mem.wave.z, mem.wave.lds);
+            } else {
+                choose_team<64, DT>(g, x, mem.team);
+            }
+        }
+        if (++w == n) { w = 0; ++b; }
+    }
+}
+
+// ------------------------------------------------------------------------------------------- very many classes, in chunks
+// Four launches over chunks of a block (top -> bins -> collect) and over blocks (finish).  Weights are integers, so that the
+// sums over chunks have no order.  Between the launches, for every wide block and in `ws`:
+constexpr int WT = 256, WIDE_BINS = 256, WIDE_LIST = 8192, WIDE_CHUNK = 4096, WIDE_CHUNKS = 1024;
+struct Wide {
+    char* ws;
+    int chunk, chunks;                        // classes of a chunk, chunks of the widest block
+    int per_row;                              // wide blocks a row can have
+    long long stride;                         // bytes of a block
+    bool k, p;                                // some block may have top-k / top-p
+};
+struct WideWs {
+    float* range;                             // [chunks][2] largest and smallest logit above -inf (NaN: the chunk holds one)
+    unsigned* count;                          // [chunks][WIDE_BINS] classes
+    u64* mass;                                // [chunks][WIDE_BINS] and their mass
+    u64* sum;                                 // [chunks] mass that is kept whatever the edge's bin yields
+    unsigned* any;                            // [chunks] classes with such mass
+    unsigned* listed;                         // places in the list
+    u64* list;                                // [WIDE_LIST] places in the edges' bins
+};
+long long wide_bytes(int chunks) { return 16 + 24LL * chunks + (long long)chunks * WIDE_BINS * 12 + 8LL * WIDE_LIST; }
+__device__ __forceinline__ WideWs wide_ws(const Wide& w, long long block) {
+    char* p = w.ws + block * w.stride;
+    WideWs s;
+    s.listed = (unsigned*)p; p += 16;
+    s.sum = (u64*)p; p += 8LL * w.chunks;
+    s.range = (float*)p; p += 8LL * w.chunks;
+    s.any = (unsigned*)p; p += 8LL * w.chunks;
+    s.mass = (u64*)p; p += (long long)w.chunks * WIDE_BINS * 8;
+    s.list = (u64*)p; p += 8LL * WIDE_LIST;
+    s.count = (unsigned*)p;
+    return s;
+}
+// The n-th wide feature, or -1.  Every thread of the workgroup calls it.
+__device__ __forceinline__ int wide_feature(const Choice& g, int n, int* s_n) {
+    if (g.m == 1) return n == 0 && g.sumK > g.wide_from && classes_of(g, 0) > g.wide_from ? 0 : -1;
+    if (threadIdx.x < 64) {
+        const int lane = threadIdx.x;
+        int found = -1;
+        for (int f0 = 0; f0 < g.m && found < 0; f0 += 64) {
+            u64 who = __ballot(f0 + lane < g.m && classes_of(g, min(f0 + lane, g.m - 1)) > g.wide_from);
+            const int c = (int)__popcll(who);
+            if (n < c) {
+                for (int k = 0; k < n; ++k) who &= who - 1;
+                found = f0 + (int)__builtin_ctzll(who);
+            }
+            n -= c;
+        }
+        if (lane == 0) *s_n = found;
+    }
+    __syncthreads();
+    return *s_n;
+}
+struct WideBlock {
+    Block x;
+    WideWs s;
+    int chunks;                               // of this block
+    float top, bottom;
+    bool none;
+    double scale;
+    float inv;
+};
+// Block and, from the chunks' ranges on (`ranges`), what they say of it
+__device__ __forceinline__ bool wide_block(const Choice& g, const Wide& w, long long block, bool ranges, WideBlock& o, int* s_n, TeamLds& t) {
+    const int b = (int)(block / w.per_row);
+    const int f = wide_feature(g, (int)(block - (long long)b * w.per_row), s_n);
+    if (f < 0) return false;
+    o.x = block_of(g, b, f, first_of(g, f), classes_of(g, f));
+    o.s = wide_ws(w, block);
+    o.chunks = (o.x.K + w.chunk - 1) / w.chunk;
+    o.scale = unit_scale(o.x.K);
+    if (!ranges) return true;
+    float top = -INFINITY, bottom = INFINITY;
+    u64 bad = 0, nan;
+    for (int i = threadIdx.x; i < o.chunks; i += WT) {
+        const float hi = o.s.range[2 * i], lo = o.s.range[2 * i + 1];
+        bad += hi != hi;
+        top = fmaxf(top, hi);
+        bottom = fminf(bottom, lo);
+    }
+    team_scan<WT>(bad, t, nan);
+    top = group_max<64>(top);
+    bottom = -group_max<64>(-bottom);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) t.part[threadIdx.x >> 6] = (u64)__float_as_uint(top) << 32 | __float_as_uint(bottom);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WT / 64; ++i) {
+        top = fmaxf(top, __uint_as_float((unsigned)(t.part[i] >> 32)));
+        bottom = fminf(bottom, __uint_as_float((unsigned)t.part[i]));
+    }
+    o.top = top;
+    o.bottom = bottom;
+    o.none = nan || o.x.bad || top == -INFINITY;
+    o.inv = bins_per_unit(top, bottom, o.x.T, (float)WIDE_BINS);
+    return true;
+}
+__device__ __forceinline__ int wide_bin(const WideBlock& o, float z) {
+    return linear_bin(z, o.top, o.inv, WIDE_BINS);
+}
+
+template <int DT> __global__ void __launch_bounds__(WT) wide_top_kernel(Choice g, Wide w) {
+    __shared__ int s_n;
+    __shared__ TeamLds s_t;
+    WideBlock o;
+    if (!wide_block(g, w, blockIdx.y, false, o, &s_n, s_t)) return;
+    const int c = blockIdx.x, t = threadIdx.x;
+    if (c == 0 && t == 0 && (w.k || w.p)) *o.s.listed = 0;
+    if (c >= o.chunks) return;
+    float top = -INFINITY, bottom = INFINITY;
+    bool nan = false;
+    const int to = min(o.x.K, (c + 1) * w.chunk);
+#pragma unroll 4
+    for (int i = c * w.chunk + t; i < to; i += WT) {
+        const float z = load1<DT>(g.z, o.x.at + i);
+        nan |= z != z;
+        top = fmaxf(top, z);
+        bottom = z == -INFINITY ? bottom : fminf(bottom, z);
+    }
+    top = group_max<64>(top);
+    bottom = -group_max<64>(-bottom);
+    if (__any(nan)) top = no_number();
+    if ((t & 63) == 0) s_t.part[t >> 6] = (u64)__float_as_uint(top) << 32 | __float_as_uint(bottom);
+    __syncthreads();
+    if (t == 0) {
+        for (int i = 1; i < WT / 64; ++i) {
+            const float v = __uint_as_float((unsigned)(s_t.part[i] >> 32));
+            top = top != top || v != v ? no_number() : fmaxf(top, v);
+            bottom = fminf(bottom, __uint_as_float((unsigned)s_t.part[i]));
+        }
+        o.s.range[2 * c] = top;
+        o.s.range[2 * c + 1] = bottom;
+    }
+}
+
+template <int DT> __global__ void __launch_bounds__(WT) wide_bins_kernel(Choice g, Wide w) {
+    __shared__ int s_n;
+    __shared__ TeamLds s_t;
+    WideBlock o;
+    if (!wide_block(g, w, blockIdx.y, true, o, &s_n, s_t)) return;
+    const int c = blockIdx.x, t = threadIdx.x;
+    if (c >= o.chunks || o.none) return;
+    s_t.weight[t] = 0;
+    s_t.count[t] = 0;
+    __syncthreads();
+    const int to = min(o.x.K, (c + 1) * w.chunk);
+    const bool mass = o.x.top_p < 1.0, count = o.x.top_k > 0;
+#pragma unroll 4
+    for (int i = c * w.chunk + t; i < to; i += WT) {
+        const float z = load1<DT>(g.z, o.x.at + i);
+        if (z > -INFINITY) {
+            const int bin = wide_bin(o, z);
+            if (mass) atomicAdd(&s_t.weight[bin], units(mass_of(z, o.top, o.x.c), o.scale));
+            if (count) atomicAdd(&s_t.count[bin], 1u);
+        }
+    }
+    __syncthreads();
+    o.s.mass[c * WIDE_BINS + t] = s_t.weight[t];
+    o.s.count[c * WIDE_BINS + t] = s_t.count[t];
+}
+
+// Which bins the edges fall into.  Top-k's is exact; the mass that top-k leaves is known up to its bin, so top-p's goal is one
+// of a range, and its bin too.
+struct Cut {
+    int k_bin;                                // bin of top-k's edge; WIDE_BINS: none
+    u64 k_before;                             // classes in the bins before it
+    u64 m_before, m_with;                     // mass in the bins before it, and with it
+    int p_from, p_to;                         // bins that top-p's edge can fall into; p_from > p_to: none
+    int sure;                                 // the bins before this one are kept
+};
+__device__ __forceinline__ Cut wide_cut(const Wide& w, const WideBlock& o, u64* s_mass, Cut* s_cut, TeamLds& s) {
+    const int t = threadIdx.x;
+    const bool k = o.x.top_k > 0 && o.x.top_k < o.x.K, p = o.x.top_p < 1.0;
+    u64 count = 0, mass = 0, total_count, total;
+    if (k)
+        for (int c = 0; c < o.chunks; ++c) count += o.s.count[c * WIDE_BINS + t];
+    if (p)
+        for (int c = 0; c < o.chunks; ++c) mass += o.s.mass[c * WIDE_BINS + t];
+    const u64 crun = team_scan<WT>(count, s, total_count), mrun = team_scan<WT>(mass, s, total);
+    s_mass[t] = mrun;
+    if (t == 0) *s_cut = Cut{WIDE_BINS, 0, total, total, 0, -1, WIDE_BINS};
+    __syncthreads();
+    if (k && crun >= (u64)o.x.top_k && crun - count < (u64)o.x.top_k) {
+        s_cut->k_bin = t;
+        s_cut->k_before = crun - count;
+        s_cut->m_before = mrun - mass;
+        s_cut->m_with = mrun;
+        s_cut->sure = t;
+    }
+    __syncthreads();
+    if (p) {
+        const double lo = o.x.top_p * (double)s_cut->m_before, hi = o.x.top_p * (double)s_cut->m_with;
+        const double before = (double)(mrun - mass), with = (double)mrun;
+        // the first bin at which the running mass reaches each end of the goal's range
+        if (with >= lo && (t == 0 || before < lo)) { s_cut->p_from = t; }
+        if (with >= hi && (t == 0 || before < hi)) { s_cut->p_to = t; }
+    }
+    __syncthreads();
+    Cut c = *s_cut;
+    if (p) c.sure = min(c.sure, c.p_from);
+    return c;
+}
+
+template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choice g, Wide w) {
+    __shared__ int s_n;
+    __shared__ TeamLds s_t;
+    __shared__ u64 s_mass[WIDE_BINS];
+    __shared__ Cut s_cut;
+    __shared__ u64 s_list[1024];
+    __shared__ unsigned s_listed, s_base;
+    WideBlock o;
+    if (!wide_block(g, w, blockIdx.y, true, o, &s_n, s_t)) return;
+    const int c = blockIdx.x, t = threadIdx.x;
+    if (c >= o.chunks || o.none) return;
+    const Cut cut = wide_cut(w, o, s_mass, &s_cut, s_t);
+    if (t == 0) s_listed = 0;
+    __syncthreads();
+    const int to = min(o.x.K, (c + 1) * w.chunk);
+    u64 sum = 0, any = 0;
+#pragma unroll 4
+    for (int i = c * w.chunk + t; i < to; i += WT) {
+        const float z = load1<DT>(g.z, o.x.at + i);
+        if (!(z > -INFINITY)) continue;
+        const int bin = wide_bin(o, z);
+        if (bin == cut.k_bin || (bin >= cut.p_from && bin <= cut.p_to)) {
+            const unsigned at = atomicAdd(&s_listed, 1u);
+            const u64 place = place_of(key_of(z), (unsigned)i);
+            if (at < 1024) s_list[at] = place;
+            else {                                            // more than a chunk usually has
+                const unsigned far = atomicAdd(o.s.listed, 1u);
+                if (far < WIDE_LIST) o.s.list[far] = place;
+            }
+        } else if (bin < cut.sure) {
+            const double a = mass_of(z, o.top, o.x.c);
+            if (a >= o.x.min_p) { sum += units(a, o.scale); any += a > 0.0; }
+        }
+    }
+    u64 total, n_any;
+    team_scan<WT>(sum, s_t, total);
+    team_scan<WT>(any, s_t, n_any);
+    const unsigned n = min(s_listed, 1024u);
+    if (t == 0) {
+        o.s.sum[c] = total;
+        o.s.any[c] = (unsigned)n_any;
+        s_base = n ? atomicAdd(o.s.listed, n) : 0;
+    }
+    __syncthreads();
+    for (unsigned i = t; i < n; i += WT)
+        if (s_base + i < WIDE_LIST) o.s.list[s_base + i] = s_list[i];
+}
+
+template <int DT> __global__ void __launch_bounds__(WT) wide_finish_kernel(Choice g, Wide w) {
+    __shared__ int s_n;
+    __shared__ TeamLds s_t;
+    __shared__ u64 s_mass[WIDE_BINS];
+    __shared__ Cut s_cut;
+    __shared__ u64 s_sum[WIDE_CHUNKS];
+    __shared__ int s_chunk;
+    __shared__ u64 s_before;
+    WideBlock o;
+    if (!wide_block(g, w, blockIdx.x, true, o, &s_n, s_t)) return;
+    const int t = threadIdx.x;
+    if (o.none) {
+        if (t == 0) give(g, o.x.b, o.x.f, -1, no_number());
+        return;
+    }
+    const Cut cut = wide_cut(w, o, s_mass, &s_cut, s_t);
+    const unsigned n = w.k || w.p ? *o.s.listed : 0;
+    if (n > WIDE_LIST) {                                      // too many classes in the edges' bins
+        choose_team<WT, DT>(g, o.x, s_t);
+        return;
+    }
+    auto z_of = [&](u64 place) {
+        const unsigned key = (unsigned)(place >> 32);
+        return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+    };
+    u64 edge = 0;
+    u64 k_mass = cut.m_before;
+    if (cut.k_bin < WIDE_BINS) {
+        edge = team_edge<WT>((double)o.x.top_k, cut.k_before, s_t, [&](auto f) {
+            for (unsigned i = t; i < n; i += WT)
+                if (wide_bin(o, z_of(o.s.list[i])) == cut.k_bin) f(o.s.list[i], 1);
+        });
+        if (cut.p_from <= cut.p_to) {
+            u64 own = 0, sum;
+            for (unsigned i = t; i < n; i += WT) {
+                const float z = z_of(o.s.list[i]);
+                if (wide_bin(o, z) == cut.k_bin && o.s.list[i] >= edge) own += units(mass_of(z, o.top, o.x.c), o.scale);
+            }
+            team_scan<WT>(own, s_t, sum);
+            k_mass += sum;
+        }
+    }
+    if (cut.p_from <= cut.p_to) {
+        const double goal = o.x.top_p * (double)k_mass;
+        const u64 before = cut.p_from ? s_mass[cut.p_from - 1] : 0;
+        const u64 to = team_edge<WT>(goal, before, s_t, [&](auto f) {
+            for (unsigned i = t; i < n; i += WT) {
+                const u64 place = o.s.list[i];
+                const int bin = wide_bin(o, z_of(place));
+                if (bin >= cut.p_from && bin <= cut.p_to && place >= edge) f(place, units(mass_of(z_of(place), o.top, o.x.c), o.scale));
+            }
+        });
+        edge = max(edge, to);
+    }
+    // the kept mass of every chunk
+    __syncthreads();
+    for (int c = t; c < o.chunks; c += WT) s_sum[c] = o.x.u == 0.0 ? (u64)o.s.any[c] : o.s.sum[c];
+    __syncthreads();
+    u64 mass = 0;
+    for (int c = t; c < o.chunks; c += WT) mass += o.s.sum[c];
+    for (unsigned i = t; i < n; i += WT) {
+        const u64 place = o.s.list[i];
+        if (place < edge) continue;
+        const double a = mass_of(z_of(place), o.top, o.x.c);
+        if (a >= o.x.min_p && a > 0.0) {
+            const u64 m = units(a, o.scale);
+            mass += m;
+            atomicAdd(&s_sum[(unsigned)~(unsigned)place / (unsigned)w.chunk], o.x.u == 0.0 ? (u64)1 : m);
+        }
+    }
+    u64 total, all;
+    team_scan<WT>(mass, s_t, total);
+    __syncthreads();
+    // the chunk in which the running mass passes the goal
+    const int per = (o.chunks + WT - 1) / WT, c0 = min(o.chunks, t * per), c1 = min(o.chunks, c0 + per);
+    u64 own = 0;
+    for (int c = c0; c < c1; ++c) own += s_sum[c];
+    u64 run = team_scan<WT>(own, s_t, all) - own;
+    const u64 goal = draw_goal(o.x.u, all);
+    if (own && run <= goal && run + own > goal) {
+        int c = c0;
+        while (c < c1 - 1 && run + s_sum[c] <= goal) run += s_sum[c++];
+        s_chunk = c;
+        s_before = run;
+    }
+    __syncthreads();
+    team_draw<WT, DT>(g, o.x, o.top, edge, o.scale, s_chunk * w.chunk, min(o.x.K, (s_chunk + 1) * w.chunk), s_before, goal, total, s_t);
+}
+
+int wide_chunk(int K) {
+    const int c = (K + WIDE_CHUNKS - 1) / WIDE_CHUNKS;
+    return c > WIDE_CHUNK ? c : WIDE_CHUNK;
+}
+constexpr int NARROW_MAX = 2048;              // classes that a wavefront keeps in LDS
+int wide_per_row(int m, int sumK) {
+    const int most = sumK / (NARROW_MAX + 1);
+    return most < m ? most : m;
+}
+// Rows of one launch: 1024 wide blocks fill the chip, and the workspace need not hold more
+int wide_rows(int per_row) { return per_row < 1024 ? 1024 / per_row : 1; }
+bool filters_k(const clava_choice* c) { return c->top_k_t || c->top_k > 0 || c->temperature_t || c->temperature < 1e-290; }
+bool filters_p(const clava_choice* c) { return c->top_p_t || c->top_p < 1.0; }
+
+template <int DT> int launch_choice(Choice& g, Wide& w, int max_k, hipStream_t st) {
+    const unsigned blocks = (unsigned)g.B * (unsigned)g.m;
+    if (!(g.wide_from && g.m == 1 && !g.offsets)) {           // else: one feature, and it is wide
+        const unsigned grid = (blocks + WAVES - 1) / WAVES < 256 * 6 ? (blocks + WAVES - 1) / WAVES : 256 * 6;
+        if (max_k <= 1024) choose_kernel<DT, 16><<<grid, WAVES * 64, 0, st>>>(g);
+        else choose_kernel<DT, 32><<<grid, WAVES * 64, 0, st>>>(g);
+        CLAVA_CHECK_LAUNCH("sample_categories");
+    }
+    if (g.wide_from) {
+        const int rows = wide_rows(w.per_row);
+        for (long long row = 0; row < g.B; row += rows) {
+            Choice h = g;                                     // the rows of this launch
+            h.z = (const char*)g.z + (size_t)row * g.ld * (DT == CLAVA_DT_F32 ? 4 : 2);
+            h.B = (int)(g.B - row < rows ? g.B - row : rows);
+            h.u = g.u ? g.u + row * g.ld_u : nullptr;
+            h.row_offset = g.row_offset + (u64)row;
+            h.idx = g.idx + row * g.m;
+            h.log_prob = g.log_prob ? g.log_prob + row * g.m : nullptr;
+            if (h.p.temperature_t) h.p.temperature_t += row * h.p.temperature_rs;
+            if (h.p.top_p_t) h.p.top_p_t += row * h.p.top_p_rs;
+            if (h.p.min_p_t) h.p.min_p_t += row * h.p.min_p_rs;
+            if (h.p.top_k_t) h.p.top_k_t += row * h.p.top_k_rs;
+            const unsigned pairs = (unsigned)h.B * (unsigned)w.per_row;
+            const dim3 grid((unsigned)w.chunks, pairs);
+            wide_top_kernel<DT><<<grid, WT, 0, st>>>(h, w);
+            if (w.k || w.p) wide_bins_kernel<DT><<<grid, WT, 0, st>>>(h, w);
+            wide_collect_kernel<DT><<<grid, WT, 0, st>>>(h, w);
+            wide_finish_kernel<DT><<<pairs, WT, 0, st>>>(h, w);
+            CLAVA_CHECK_LAUNCH("sample_categories (wide)");
+        }
+    }
+    return CLAVA_OK;
 }
 
 }  // namespace
 
 extern "C" {
 
-long long clava_choice_workspace_bytes(int, int, int) { return 0; }
+long long clava_choice_workspace_bytes(int B, int m, int sumK, int max_k) {
+    if (B <= 0 || m <= 0 || sumK <= NARROW_MAX || max_k <= NARROW_MAX) return 0;
+    const int chunk = wide_chunk(sumK), chunks = (sumK + chunk - 1) / chunk;
+    const int per_row = wide_per_row(m, sumK), rows = wide_rows(per_row);
+    return (long long)(B < rows ? B : rows) * per_row * ((wide_bytes(chunks) + 15) / 16 * 16);
+}
 
 int clava_sample_categories(const void* logits, int dtype, long long ld, int B, int m, int sumK, const int* offsets, int max_k,
                             const clava_choice* choice, const float* uniforms, long long ld_u, unsigned long long seed,
@@ -223,20 +1145,33 @@ int clava_sample_categories(const void* logits, int dtype, long long ld, int B, 
     CLAVA_CHECK_ARG(dtype >= 0 && dtype <= CLAVA_DT_F16, "sample_categories: dtype %d", dtype);
     CLAVA_CHECK_ARG(ld >= sumK || B == 1, "sample_categories: leading dimension %lld below %d classes", ld, sumK);
     CLAVA_CHECK_ARG(!uniforms || ld_u >= m || B == 1, "sample_categories: leading dimension %lld below %d uniforms", ld_u, m);
-    CLAVA_CHECK_ARG(sumK <= (1 << 30), "sample_categories: %d classes", sumK);
+    if (sumK > (1 << 30) || (long long)B * m > 0x7fffffffLL || wide_per_row(m, sumK) > 65535) {
+        clava_set_error("sample_categories: %d rows of %d features and %d classes are more than one call takes", B, m, sumK);
+        return CLAVA_ERR_LIMIT;
+    }
+    const long long need = clava_choice_workspace_bytes(B, m, sumK, max_k);
+    CLAVA_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+                    "sample_categories: needs a 16-byte aligned workspace of %lld bytes, got %lld", need, workspace_bytes);
     const hipStream_t st = (hipStream_t)stream;
     Choice g;
     g.z = logits; g.ld = ld; g.B = B; g.m = m; g.sumK = sumK; g.offsets = offsets; g.p = *choice;
+    g.c = LOG2E / choice->temperature;
     g.u = uniforms; g.ld_u = ld_u; g.seed = seed; g.row_offset = row_offset; g.step = step_index;
     g.idx = idx; g.log_prob = log_prob;
-    const long long blocks = (long long)B * m;
-    const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
-    ProfScope prof(PROF_CHOICE, 0, (double)B * sumK * (dtype == CLAVA_DT_F32 ? 4 : 2) + 12.0 * blocks, st);
-    if (dtype == CLAVA_DT_F32) choose_kernel<CLAVA_DT_F32><<<grid, W, 0, st>>>(g);
-    else if (dtype == CLAVA_DT_BF16) choose_kernel<CLAVA_DT_BF16><<<grid, W, 0, st>>>(g);
-    else choose_kernel<CLAVA_DT_F16><<<grid, W, 0, st>>>(g);
-    CLAVA_CHECK_LAUNCH("sample_categories");
-    return CLAVA_OK;
+    g.wide_from = need ? NARROW_MAX : 0;
+    Wide w{};
+    if (need) {
+        w.ws = (char*)workspace;
+        w.chunk = wide_chunk(sumK);
+        w.chunks = (sumK + w.chunk - 1) / w.chunk;
+        w.per_row = wide_per_row(m, sumK);
+        w.stride = (wide_bytes(w.chunks) + 15) / 16 * 16;
+        w.k = filters_k(choice);
+        w.p = filters_p(choice);
+    }
+    ProfScope prof(PROF_CHOICE, 0, (double)B * sumK * (dtype == CLAVA_DT_F32 ? 4 : 2) + 12.0 * B * m, st);
+    return dtype == CLAVA_DT_F32 ? launch_choice<CLAVA_DT_F32>(g, w, max_k, st)
+           : dtype == CLAVA_DT_BF16 ? launch_choice<CLAVA_DT_BF16>(g, w, max_k, st) : launch_choice<CLAVA_DT_F16>(g, w, max_k, st);
 }
 
 }  // extern "C"

@@ -505,7 +505,7 @@ def sample_categories(logits, uniforms=None, offsets=None, max_classes=None, *, 
     lp = torch.empty((B, m), device=dev, dtype=torch.float32) if log_prob else None
     L = lib()
     L.clava_choice_workspace_bytes.restype = c_ll
-    need = L.clava_choice_workspace_bytes(c_int(B), c_int(m), c_int(max_classes))
+    need = L.clava_choice_workspace_bytes(c_int(B), c_int(m), c_int(sumk), c_int(max_classes))
     with _on(dev):
         ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
         check(L.clava_sample_categories(ptr(logits), dt, c_ll(_rs(logits)), c_int(B), c_int(m), c_int(sumk), ptr(offsets), c_int(max_classes),

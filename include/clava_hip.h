@@ -242,7 +242,7 @@ int clava_categorical_sampler_set(int mode);
  * Each parameter is a number for all blocks, or, where its pointer is not NULL, element [b * rs + f * fs] of a device array.
  * uniforms [b * ld_u + f] in [0, 1), or NULL for the counter-based generator keyed by (seed, row_offset + b, f, step_index).
  * max_k: the largest number of classes of one feature (a hint that picks the kernels; any value is safe).  workspace:
- * clava_choice_workspace_bytes(B, m, max_k) bytes, 16-byte aligned (may be NULL where that is 0); its contents need not be kept. */
+ * clava_choice_workspace_bytes(B, m, sumK, max_k) bytes, 16-byte aligned (may be NULL where that is 0); its contents need not be kept. */
 typedef struct clava_choice {
     double temperature, top_p, min_p;
     int top_k;
@@ -252,7 +252,7 @@ typedef struct clava_choice {
     const int* top_k_t;
     long long temperature_rs, temperature_fs, top_p_rs, top_p_fs, min_p_rs, min_p_fs, top_k_rs, top_k_fs;
 } clava_choice;
-long long clava_choice_workspace_bytes(int B, int m, int max_k);
+long long clava_choice_workspace_bytes(int B, int m, int sumK, int max_k);
 int clava_sample_categories(const void* logits, int dtype, long long ld, int B, int m, int sumK, const int* offsets, int max_k,
                             const clava_choice* choice, const float* uniforms, long long ld_u, unsigned long long seed,
                             unsigned long long row_offset, unsigned step_index, int* idx, float* log_prob, void* workspace,

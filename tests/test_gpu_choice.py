@@ -66,19 +66,22 @@ def offsets(classes):
     return torch.tensor(np.concatenate([[0], np.cumsum(classes)]), device=DEV, dtype=torch.int32)
 
 
-def same(got, want):
+def same(got, want, widest=0):
+    """Equal classes; log-probabilities within the float32 rounding (half a step), the float64 arithmetic's 1e-12 and, for
+    features of more than 2048 classes, what the masses lose as whole units of 2^-s, s = min(51, 62 - ceil(log2 K)): half a
+    unit a class, K 2^-(s + 1) in all, of a sum that is at least 1."""
     idx, lp = got
     assert np.array_equal(idx.cpu().numpy(), want[0])
-    # the logarithm's float32 rounding (half a step), and its float64 argument
     g, w = lp.cpu().double().numpy(), want[1]
     assert np.array_equal(np.isnan(g), np.isnan(w))
     ok = ~np.isnan(w)
-    assert (np.abs(g[ok] - w[ok]) <= np.abs(w[ok]) * 2.0 ** -24 + 1e-12).all()
+    units = widest * 2.0 ** -(min(51, 62 - math.ceil(math.log2(widest))) + 1) if widest > 2048 else 0.0
+    assert (np.abs(g[ok] - w[ok]) <= np.abs(w[ok]) * 2.0 ** -24 + 1e-12 + units).all()
 
 
 def check(logits, u, classes, max_classes=None, **p):
     got = ops.sample_categories(logits.to(DEV), u.to(DEV), offsets(classes), max_classes, log_prob=True, **p)
-    same(got, expect(logits, u, classes, **{"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0, **p}))
+    same(got, expect(logits, u, classes, **{"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0, **p}), max(classes))
     return got
 
 
@@ -174,7 +177,7 @@ def test_parameters_for_every_row_and_feature():
         for f in range(m):
             idx[b, f], lp[b, f] = choose(z64[b, at[f]:at[f + 1]], float(u[b, f]), temperature=full(t)[b, f], top_k=int(want_k[b, f]),
                                          top_p=full(p)[b, f], min_p=full(mn)[b, f])
-    same(got, (idx, lp))
+    same(got, (idx, lp), max(classes))
 
 
 def test_features_without_classes_strides_and_a_wrong_hint():
@@ -186,7 +189,7 @@ def test_features_without_classes_strides_and_a_wrong_hint():
     want = expect(z, u, classes, temperature=0.8, top_k=9, top_p=0.9, min_p=0.0)
     zd, ud = big.to(DEV)[::2, 3:3 + sum(classes)], ub.to(DEV)[:, 1:1 + len(classes)]
     for hint in (None, 0, 1, 70, 2300, 10 ** 6):
-        same(ops.sample_categories(zd, ud, offsets(classes), hint, temperature=0.8, top_k=9, top_p=0.9, log_prob=True), want)
+        same(ops.sample_categories(zd, ud, offsets(classes), hint, temperature=0.8, top_k=9, top_p=0.9, log_prob=True), want, max(classes))
     # offsets outside of the row are cut to it
     off = torch.tensor([-5, 4, 10 ** 6, 2], device=DEV, dtype=torch.int32)
     got = ops.sample_categories(zd, ud[:, :3], off)
