@@ -39,7 +39,7 @@ __device__ __forceinline__ void activate8(float* v, int act) {
 // eight neighbouring columns of y.
 __device__ __forceinline__ int pair_row(int r, int odd) { return 8 * (r >> 2) + 4 * odd + (r & 3); }
 
-constexpr int OUT_MX4 = 3;
+constexpr int OUT_MX4 = CLAVA_DT_MX4;
 __device__ __forceinline__ void bias8(const Mx4Args& g, int n0, float* b) {
     if (g.bias) load8<CLAVA_DT_F32>(g.bias, (size_t)n0, g.N - n0, b);
     else
@@ -251,27 +251,39 @@ template <int OUT> int launch_linear(const Mx4Args& g, hipStream_t st) {
 
 extern "C" {
 
-int clava_linear_mx4(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, int act,
-                     void* y, int y_dtype, long long ldy, void* y_codes, void* y_scales, int M, int N, int K, void* stream) {
+long long clava_linear_mx4_workspace_bytes(int M, int K, int x_dtype) {
+    return M > 0 && K > 0 && x_dtype != CLAVA_DT_MX4 ? (long long)M * steps(K) * 68 : 0;
+}
+
+int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_scales, const void* w_codes, const void* w_scales,
+                     const float* bias, int act, void* y, int y_dtype, long long ldy, void* y_scales, int M, int N, int K,
+                     void* workspace, void* stream) {
     CLAVA_CHECK_ARG(M >= 0 && N > 0 && K > 0, "linear_mx4: M %d, N %d, K %d", M, N, K);
     CLAVA_CHECK_ARG(act >= CLAVA_ACT_NONE && act <= CLAVA_ACT_SILU, "linear_mx4: activation %d", act);
-    CLAVA_CHECK_ARG((y != nullptr) != (y_codes != nullptr) || M == 0, "linear_mx4: one of y and y_codes");
+    CLAVA_CHECK_ARG(x_dtype >= 0 && x_dtype <= CLAVA_DT_MX4 && y_dtype >= 0 && y_dtype <= CLAVA_DT_MX4, "linear_mx4: dtypes %d, %d", x_dtype, y_dtype);
     if (M == 0) return CLAVA_OK;
-    CLAVA_CHECK_ARG(x_codes && x_scales && w_codes && w_scales && (y || y_scales), "linear_mx4: null pointer");
-    CLAVA_CHECK_ARG(!y || (y_dtype >= 0 && y_dtype <= CLAVA_DT_F16), "linear_mx4: dtype %d", y_dtype);
-    CLAVA_CHECK_ARG(!y || ldy >= N || M == 1, "linear_mx4: leading dimension %lld below %d columns", ldy, N);
-    CLAVA_CHECK_ARG(((uintptr_t)x_codes & 15) == 0 && ((uintptr_t)w_codes & 15) == 0, "linear_mx4: codes must start at 16 bytes");
+    const bool x4 = x_dtype == CLAVA_DT_MX4, y4 = y_dtype == CLAVA_DT_MX4;
+    CLAVA_CHECK_ARG(x && w_codes && w_scales && y && (!y4 || y_scales) && (x4 ? x_scales : workspace), "linear_mx4: null pointer");
+    CLAVA_CHECK_ARG(y4 || ldy >= N || M == 1, "linear_mx4: leading dimension %lld below %d columns", ldy, N);
+    CLAVA_CHECK_ARG((((uintptr_t)(x4 ? x : workspace) | (uintptr_t)w_codes) & 15) == 0, "linear_mx4: codes and workspace start at 16 bytes");
     CLAVA_CHECK_ARG(N <= 0x7fffff00 && K <= 0x7fffff00 && M <= 0x7fffff00, "linear_mx4: M %d, N %d, K %d", M, N, K);
     const hipStream_t st = (hipStream_t)stream;
     Mx4Args g;
-    g.xq = (const char*)x_codes; g.xs = (const unsigned char*)x_scales;
+    g.ks = steps(K);
+    g.xq = (const char*)x; g.xs = (const unsigned char*)x_scales;
+    if (!x4) {
+        g.xq = (const char*)workspace;
+        g.xs = (const unsigned char*)workspace + (size_t)M * g.ks * 64;
+        const int rc = clava_mx4_pack(x, x_dtype, ldx, M, K, (void*)g.xq, (void*)g.xs, stream);
+        if (rc) return rc;
+    }
     g.wq = (const char*)w_codes; g.ws = (const unsigned char*)w_scales;
     g.bias = bias; g.act = act;
     g.y = y; g.ldy = ldy;
-    g.yq = (unsigned*)y_codes; g.ys = (unsigned char*)y_scales; g.yks = steps(N);
-    g.M = M; g.N = N; g.ks = steps(K);
-    ProfScope prof(PROF_MX4, 2.0 * M * N * K, ((double)M * K + (double)N * K) * 17.0 / 32 + (double)M * N * (!y ? 17.0 / 32 : y_dtype == 0 ? 4 : 2), st);
-    const int rc = !y ? launch_linear<OUT_MX4>(g, st)
+    g.yq = (unsigned*)y; g.ys = (unsigned char*)y_scales; g.yks = steps(N);
+    g.M = M; g.N = N;
+    ProfScope prof(PROF_MX4, 2.0 * M * N * K, ((double)M * K + (double)N * K) * 17.0 / 32 + (double)M * N * (y4 ? 17.0 / 32 : y_dtype == 0 ? 4 : 2), st);
+    const int rc = y4 ? launch_linear<OUT_MX4>(g, st)
                       : y_dtype == CLAVA_DT_F32 ? launch_linear<CLAVA_DT_F32>(g, st)
                       : y_dtype == CLAVA_DT_BF16 ? launch_linear<CLAVA_DT_BF16>(g, st) : launch_linear<CLAVA_DT_F16>(g, st);
     if (rc) return rc;

@@ -4,7 +4,6 @@ Only plumbing lives here: argument checking, output allocation through torch's
 caching allocator, and the raw-pointer call.  All arithmetic is in the HIP
 library.
 """
-import contextlib
 import ctypes
 import math
 
@@ -299,61 +298,94 @@ def linear_f16x3(x, w, bias=None, act=None, rowadd=None, act_out=None, slope=0.0
 
 
 # ---- microscaled 4-bit matrices (OCP MX, E2M1 over blocks of 32 columns) and dense layers over them --------------------
+# These calls take a few microseconds on the GPU at their smallest, so their host side counts: C functions with declared
+# argument types (plain Python numbers, no ctypes objects), one look at a tensor's shape and strides.
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MX4 = 3
 c_ll = ctypes.c_longlong
+_C_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": c_ll, "u": ctypes.c_uint, "U": ctypes.c_ulonglong}
+_FUNCTIONS = {}
+
+
+def _function(name, types, result=ctypes.c_int):
+    f = _FUNCTIONS.get(name)
+    if f is None:
+        f = getattr(lib(), name)
+        f.argtypes = [_C_TYPES[c] for c in types]
+        f.restype = result
+        _FUNCTIONS[name] = f
+    return f
+
+
+def _refuse(message):
+    raise _lib.ClavaHipError(message)
 
 
 def _dt(t, name):
-    if t.dtype not in _DT:
-        raise _lib.ClavaHipError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    return c_int(_DT[t.dtype])
+    d = _DT.get(t.dtype)
+    if d is None:
+        _refuse(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return d
 
 
 def _matrix(t, name):
-    """A [rows, cols] device tensor with contiguous rows."""
-    require_cuda(t)
+    """(rows, columns, row stride) of a device tensor [rows, cols] with contiguous rows."""
+    if not t.is_cuda:
+        require_cuda(t)
     if t.dim() != 2:
-        raise _lib.ClavaHipError(f"{name}: expected [rows, cols], got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise _lib.ClavaHipError(f"{name}: innermost dimension must be contiguous")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise _lib.ClavaHipError(f"{name}: rows overlap (stride {t.stride(0)} for {t.shape[1]} columns)")
-    return t
+        _refuse(f"{name}: expected [rows, cols], got {tuple(t.shape)}")
+    (rows, cols), (ld, inner) = t.shape, t.stride()
+    if inner != 1 and cols > 1:
+        _refuse(f"{name}: innermost dimension must be contiguous")
+    if rows > 1:
+        if ld < cols:
+            _refuse(f"{name}: rows overlap (stride {ld} for {cols} columns)")
+    elif ld < cols:
+        ld = cols                  # (torch reports any stride for a single row)
+    return rows, cols, ld
 
 
 def _same_device(dev, **tensors):
     for name, t in tensors.items():
         if t is not None and t.device != dev:
-            raise _lib.ClavaHipError(f"{name} is on {t.device}, expected {dev}")
+            _refuse(f"{name} is on {t.device}, expected {dev}")
 
 
-def _on(dev):
-    """The tensors' device as the current one, where it is not: launches go to its current stream."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _launch(dev, name, f, *args):
+    """f(*args, stream) on the current stream of the tensors' device."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
 
 
 class Mx4Tensor:
     """A [rows, cols] matrix in microscaled 4-bit form (see include/clava_hip.h): `codes` uint8 [rows, Kp / 2] and `scales`
     uint8 [rows, Kp / 32], Kp = cols rounded up to 128.  The codes behind the last column have to be zero."""
-    __slots__ = ("codes", "scales", "rows", "cols")
+    __slots__ = ("codes", "scales", "rows", "cols", "device")
 
     def __init__(self, codes, scales, cols):
-        require_cuda(codes, scales)
-        rows, cols = codes.shape[0], int(cols)
-        kp = (cols + 127) // 128 * 128
+        cols = int(cols)
+        steps = (cols + 127) // 128
         if cols < 1:
-            raise _lib.ClavaHipError(f"Mx4Tensor: {cols} columns")
-        for name, t, width in (("codes", codes, kp // 2), ("scales", scales, kp // 32)):
-            if t.dtype != torch.uint8 or tuple(t.shape) != (rows, width) or not t.is_contiguous():
-                raise _lib.ClavaHipError(f"Mx4Tensor: {name} must be contiguous uint8 [{rows}, {width}], got {t.dtype} {tuple(t.shape)}")
-        _same_device(codes.device, scales=scales)
-        if codes.data_ptr() % 16:
-            raise _lib.ClavaHipError("Mx4Tensor: codes must start at a multiple of 16 bytes")
+            _refuse(f"Mx4Tensor: {cols} columns")
+        rows = codes.shape[0]
+        if codes.shape != (rows, 64 * steps) or codes.dtype is not torch.uint8 or not codes.is_contiguous():
+            _refuse(f"Mx4Tensor: codes must be contiguous uint8 [{rows}, {64 * steps}], got {codes.dtype} {tuple(codes.shape)}")
+        if scales.shape != (rows, 4 * steps) or scales.dtype is not torch.uint8 or not scales.is_contiguous():
+            _refuse(f"Mx4Tensor: scales must be contiguous uint8 [{rows}, {4 * steps}], got {scales.dtype} {tuple(scales.shape)}")
+        if not codes.is_cuda:
+            require_cuda(codes)
+        self.device = codes.device
+        if scales.device != self.device:
+            _refuse(f"Mx4Tensor: scales are on {scales.device}, codes on {self.device}")
+        if codes.data_ptr() & 15:
+            _refuse("Mx4Tensor: codes must start at a multiple of 16 bytes")
         self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
-
-    @property
-    def device(self):
-        return self.codes.device
 
 
 def mx4_empty(rows, cols, device):
@@ -365,18 +397,15 @@ def mx4_empty(rows, cols, device):
 
 def mx4_pack(x, out=None):
     """[rows, cols] float32 / bfloat16 / float16 -> Mx4Tensor (clava_mx4_pack); `out` reuses one of the same shape.  A block
-    that holds a NaN or an infinity reads as NaN."""
-    x = _matrix(x, "mx4_pack: x")
-    rows, cols = x.shape
+    that holds a NaN or an infinity reads as NaN.  No gradient is defined."""
+    rows, cols, ld = _matrix(x, "mx4_pack: x")
     dt = _dt(x, "mx4_pack: x")
     if out is None:
         out = mx4_empty(rows, cols, x.device)
-    elif (out.rows, out.cols) != (rows, cols):
-        raise _lib.ClavaHipError(f"mx4_pack: x is [{rows},{cols}] but out is [{out.rows},{out.cols}]")
-    _same_device(x.device, out=out)
-    with _on(x.device):
-        check(lib().clava_mx4_pack(ptr(x), dt, c_ll(_rs(x)), c_ll(rows), c_int(cols), ptr(out.codes), ptr(out.scales), stream_ptr()),
-              "clava_mx4_pack")
+    elif (out.rows, out.cols) != (rows, cols) or out.device != x.device:
+        _refuse(f"mx4_pack: x is [{rows},{cols}] on {x.device} but out is [{out.rows},{out.cols}] on {out.device}")
+    _launch(out.device, "clava_mx4_pack", _function("clava_mx4_pack", "pillippp"),
+            x.data_ptr(), dt, ld, rows, cols, out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
 
@@ -384,16 +413,13 @@ def mx4_unpack(q, dtype=torch.float32, out=None):
     """The values of an Mx4Tensor as float32, bfloat16 or float16 (clava_mx4_unpack)."""
     if out is None:
         if dtype not in _DT:
-            raise _lib.ClavaHipError(f"mx4_unpack: expected float32, bfloat16 or float16, got {dtype}")
+            _refuse(f"mx4_unpack: expected float32, bfloat16 or float16, got {dtype}")
         out = torch.empty((q.rows, q.cols), device=q.device, dtype=dtype)
-    else:
-        out = _matrix(out, "mx4_unpack: out")
-        if tuple(out.shape) != (q.rows, q.cols):
-            raise _lib.ClavaHipError(f"mx4_unpack: q is [{q.rows},{q.cols}] but out is {tuple(out.shape)}")
-        _same_device(q.device, out=out)
-    with _on(q.device):
-        check(lib().clava_mx4_unpack(ptr(q.codes), ptr(q.scales), c_ll(q.rows), c_int(q.cols), ptr(out), _dt(out, "mx4_unpack: out"),
-                                     c_ll(_rs(out)), stream_ptr()), "clava_mx4_unpack")
+    rows, cols, ld = _matrix(out, "mx4_unpack: out")
+    if (rows, cols) != (q.rows, q.cols) or out.device != q.device:
+        _refuse(f"mx4_unpack: q is [{q.rows},{q.cols}] on {q.device} but out is [{rows},{cols}] on {out.device}")
+    _launch(q.device, "clava_mx4_unpack", _function("clava_mx4_unpack", "pplipilp"),
+            q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(), _dt(out, "mx4_unpack: out"), ld)
     return out
 
 
@@ -402,34 +428,49 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
     matrix, which is packed first.  The result is a float matrix of `out_dtype`, or whatever `out` is: a float matrix or an
     Mx4Tensor (the next layer's operand).  No gradient is defined."""
     if not isinstance(w, Mx4Tensor):
-        raise _lib.ClavaHipError("linear_mx4: w must be an Mx4Tensor")
-    if act not in _ACT:
-        raise _lib.ClavaHipError(f"linear_mx4: unknown activation {act!r}")
-    M, K = (x.rows, x.cols) if isinstance(x, Mx4Tensor) else _matrix(x, "linear_mx4: x").shape
-    N = w.rows
+        _refuse("linear_mx4: w must be an Mx4Tensor")
+    code = _ACT.get(act)
+    if code is None:
+        _refuse(f"linear_mx4: unknown activation {act!r}")
+    N, dev, ws = w.rows, w.device, None
+    if isinstance(x, Mx4Tensor):
+        M, K, ldx, x_dt, xp, xs = x.rows, x.cols, 0, _MX4, x.codes.data_ptr(), x.scales.data_ptr()
+    else:
+        M, K, ldx = _matrix(x, "linear_mx4: x")
+        x_dt, xp, xs = _dt(x, "linear_mx4: x"), x.data_ptr(), None
+        if x.requires_grad and torch.is_grad_enabled():
+            _refuse("linear_mx4 has no backward: call it under torch.no_grad() or detach its inputs")
     if w.cols != K:
-        raise _lib.ClavaHipError(f"linear_mx4: x is [{M},{K}] but w is [{w.rows},{w.cols}]")
+        _refuse(f"linear_mx4: x is [{M},{K}] but w is [{N},{w.cols}]")
     if N == 0:
-        raise _lib.ClavaHipError("linear_mx4: w has no rows")
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, bias)):
-        raise _lib.ClavaHipError("linear_mx4 has no backward: call it under torch.no_grad() or detach its inputs")
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
-        raise _lib.ClavaHipError(f"linear_mx4: bias must be contiguous float32 [{N}]")
+        _refuse("linear_mx4: w has no rows")
+    if x.device != dev:
+        _refuse(f"linear_mx4: x is on {x.device}, w on {dev}")
+    bp = None
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.shape != (N,) or not bias.is_contiguous() or bias.device != dev:
+            _refuse(f"linear_mx4: bias must be contiguous float32 [{N}] on {dev}")
+        if bias.requires_grad and torch.is_grad_enabled():
+            _refuse("linear_mx4 has no backward: call it under torch.no_grad() or detach its inputs")
+        bp = bias.data_ptr()
     if out is None:
         if out_dtype not in _DT:
-            raise _lib.ClavaHipError(f"linear_mx4: expected float32, bfloat16 or float16, got {out_dtype}")
-        out = torch.empty((M, N), device=w.device, dtype=out_dtype)
-    y4 = isinstance(out, Mx4Tensor)
-    if ((out.rows, out.cols) if y4 else tuple(_matrix(out, "linear_mx4: out").shape)) != (M, N):
-        raise _lib.ClavaHipError(f"linear_mx4: the result is [{M},{N}] but out has another shape")
-    _same_device(w.device, x=x, bias=bias, out=out)
-    if not isinstance(x, Mx4Tensor):
-        x = mx4_pack(x)
-    with _on(w.device):
-        check(lib().clava_linear_mx4(ptr(x.codes), ptr(x.scales), ptr(w.codes), ptr(w.scales), ptr(bias), c_int(_ACT[act]),
-                                     None if y4 else ptr(out), c_int(0) if y4 else _dt(out, "linear_mx4: out"), c_ll(0 if y4 else _rs(out)),
-                                     ptr(out.codes) if y4 else None, ptr(out.scales) if y4 else None, c_int(M), c_int(N), c_int(K),
-                                     stream_ptr()), "clava_linear_mx4")
+            _refuse(f"linear_mx4: expected float32, bfloat16 or float16, got {out_dtype}")
+        out = torch.empty((M, N), device=dev, dtype=out_dtype)
+        y_dt, ldy, yp, ys = _DT[out_dtype], N, out.data_ptr(), None
+    else:
+        if isinstance(out, Mx4Tensor):
+            rows, cols, ldy, y_dt, yp, ys = out.rows, out.cols, 0, _MX4, out.codes.data_ptr(), out.scales.data_ptr()
+        else:
+            rows, cols, ldy = _matrix(out, "linear_mx4: out")
+            y_dt, yp, ys = _dt(out, "linear_mx4: out"), out.data_ptr(), None
+        if (rows, cols) != (M, N) or out.device != dev:
+            _refuse(f"linear_mx4: the result is [{M},{N}] on {dev} but out is [{rows},{cols}] on {out.device}")
+    if x_dt != _MX4:
+        ws = torch.empty(M * 68 * ((K + 127) // 128), device=dev, dtype=torch.uint8)      # clava_linear_mx4_workspace_bytes
+    _launch(dev, "clava_linear_mx4", _function("clava_linear_mx4", "pilppppipilpiiipp"),
+            xp, x_dt, ldx, xs, w.codes.data_ptr(), w.scales.data_ptr(), bp, code, yp, y_dt, ldy, ys, M, N, K,
+            None if ws is None else ws.data_ptr())
     return out
 
 
@@ -440,77 +481,77 @@ class _CChoice(ctypes.Structure):
                [(n + s, c_ll) for n in ("temperature", "top_p", "min_p", "top_k") for s in ("_rs", "_fs")]
 
 
-def _choice_args(dev, rows, features, **values):
+_CHOICE_RANGE = {"temperature": (0.0, math.inf), "top_p": (0.0, math.inf), "min_p": (0.0, 1.0), "top_k": (-math.inf, math.inf)}
+
+
+def _choice_args(dev, rows, features, values):
     """The C struct of the four parameters: numbers, or tensors that broadcast to [rows, features]."""
     c = _CChoice()
-    keep = []
-    for name, v in values.items():
-        want = torch.int32 if name == "top_k" else torch.float32
-        if not isinstance(v, torch.Tensor):
-            low, high = {"temperature": (0.0, math.inf), "top_p": (0.0, math.inf), "min_p": (0.0, 1.0), "top_k": (-math.inf, math.inf)}[name]
-            if not low <= v <= high:
-                raise _lib.ClavaHipError(f"sample_categories: {name} {v} outside [{low}, {high}]")
-            setattr(c, name, max(-1, min(int(v), 2 ** 31 - 1)) if name == "top_k" else float(v))
+    for name, v in values:
+        if isinstance(v, torch.Tensor):
+            want = torch.int32 if name == "top_k" else torch.float32
+            if v.dtype is not want or v.device != dev:
+                _refuse(f"sample_categories: {name} must be {want} on {dev}, got {v.dtype} on {v.device}")
+            try:
+                v = v.expand(rows, features)
+            except RuntimeError:
+                raise _lib.ClavaHipError(f"sample_categories: {name} {tuple(v.shape)} does not broadcast to [{rows},{features}]") from None
+            setattr(c, name + "_t", v.data_ptr())
+            rs, fs = v.stride()
+            setattr(c, name + "_rs", rs)
+            setattr(c, name + "_fs", fs)
             continue
-        _same_device(dev, **{name: v})
-        if v.dtype != want:
-            raise _lib.ClavaHipError(f"sample_categories: {name} must be {want}, got {v.dtype}")
-        try:
-            v = v.expand(rows, features)
-        except RuntimeError:
-            raise _lib.ClavaHipError(f"sample_categories: {name} {tuple(v.shape)} does not broadcast to [{rows},{features}]") from None
-        keep.append(v)
-        setattr(c, name + "_t", v.data_ptr())
-        setattr(c, name + "_rs", v.stride(0))
-        setattr(c, name + "_fs", v.stride(1))
-    return c, keep
+        low, high = _CHOICE_RANGE[name]
+        if not low <= v <= high:
+            _refuse(f"sample_categories: {name} {v} outside [{low}, {high}]")
+        setattr(c, name, max(-1, min(int(v), 2 ** 31 - 1)) if name == "top_k" else v)
+    return c
 
 
 def sample_categories(logits, uniforms=None, offsets=None, max_classes=None, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
                       log_prob=False, seed=0, row_offset=0, step_index=0, out=None):
     """One class per (row, feature) from `logits` [B, sumK] (float32, bfloat16 or float16) with temperature, top-k, top-p and
     min-p, as clava_sample_categories defines them; int32 [B, m], with `log_prob` also the log-probability of every drawn class
-    under the filtered distribution, float32 [B, m].
+    under the filtered distribution, float32 [B, m] (no gradient is defined).
 
     Feature f owns columns offsets[f] .. offsets[f+1] (int32 device tensor [m + 1]; None: one feature of all columns).
     `uniforms`: float32 [B, m] in [0, 1) ([B] for one feature), or None for the generator keyed by (seed, row_offset + row,
     feature, step_index).  `max_classes`: the largest number of classes of one feature, which picks the kernels (any value is
     safe; default: all columns).  Each parameter is a number or a device tensor (float32; top_k int32) that broadcasts to
     [B, m].  A feature with no class left to draw (none, all logits -inf, a NaN) yields -1 and NaN."""
-    logits = _matrix(logits, "sample_categories: logits")
+    B, sumk, ld = _matrix(logits, "sample_categories: logits")
     dt = _dt(logits, "sample_categories: logits")
-    B, sumk = logits.shape
     dev = logits.device
-    m = 1
+    m, op = 1, None
     if offsets is not None:
-        if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 2 or not offsets.is_contiguous():
-            raise _lib.ClavaHipError("sample_categories: offsets must be contiguous int32 [m + 1]")
-        m = offsets.numel() - 1
-    ld_u = 0
+        if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2 or not offsets.is_contiguous() or offsets.device != dev:
+            _refuse(f"sample_categories: offsets must be contiguous int32 [m + 1] on {dev}")
+        m, op = offsets.shape[0] - 1, offsets.data_ptr()
+    ld_u, up = 0, None
     if uniforms is not None:
-        if uniforms.dtype != torch.float32 or tuple(uniforms.shape) not in ((B, m),) + (((B,),) if m == 1 else ()):
-            raise _lib.ClavaHipError(f"sample_categories: uniforms must be float32 [{B},{m}], got {uniforms.dtype} {tuple(uniforms.shape)}")
-        uniforms = _matrix(uniforms.reshape(B, m) if uniforms.dim() == 1 else uniforms, "sample_categories: uniforms")
-        ld_u = _rs(uniforms)
+        if uniforms.dim() == 1 and m == 1:
+            uniforms = uniforms.reshape(-1, 1)
+        rows, cols, ld_u = _matrix(uniforms, "sample_categories: uniforms")
+        if uniforms.dtype is not torch.float32 or (rows, cols) != (B, m) or uniforms.device != dev:
+            _refuse(f"sample_categories: uniforms must be float32 [{B},{m}] on {dev}, got {uniforms.dtype} [{rows},{cols}] on {uniforms.device}")
+        up = uniforms.data_ptr()
     if max_classes is None or max_classes > sumk:
         max_classes = sumk
-    if max_classes < 0:
-        raise _lib.ClavaHipError(f"sample_categories: max_classes {max_classes}")
+    elif max_classes < 0:
+        _refuse(f"sample_categories: max_classes {max_classes}")
     if out is None:
         out = torch.empty((B, m), device=dev, dtype=torch.int32)
-    elif out.dtype != torch.int32 or tuple(out.shape) != (B, m) or not out.is_contiguous():
-        raise _lib.ClavaHipError(f"sample_categories: out must be contiguous int32 [{B},{m}]")
-    _same_device(dev, offsets=offsets, uniforms=uniforms, out=out)
-    c, keep = _choice_args(dev, B, m, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    elif out.dtype is not torch.int32 or out.shape != (B, m) or not out.is_contiguous() or out.device != dev:
+        _refuse(f"sample_categories: out must be contiguous int32 [{B},{m}] on {dev}")
+    c = _choice_args(dev, B, m, (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)))
     lp = torch.empty((B, m), device=dev, dtype=torch.float32) if log_prob else None
-    L = lib()
-    L.clava_choice_workspace_bytes.restype = c_ll
-    need = L.clava_choice_workspace_bytes(c_int(B), c_int(m), c_int(sumk), c_int(max_classes))
-    with _on(dev):
-        ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-        check(L.clava_sample_categories(ptr(logits), dt, c_ll(_rs(logits)), c_int(B), c_int(m), c_int(sumk), ptr(offsets), c_int(max_classes),
-                                        ctypes.byref(c), ptr(uniforms), c_ll(ld_u), _lib.c_u64(seed), _lib.c_u64(row_offset),
-                                        ctypes.c_uint(step_index), ptr(out), ptr(lp), ptr(ws), c_ll(need), stream_ptr()),
-              "clava_sample_categories")
-    del keep
+    need, ws = 0, None
+    if max_classes > 2048:
+        need = _function("clava_choice_workspace_bytes", "iiii", c_ll)(B, m, sumk, max_classes)
+        if need:
+            ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    _launch(dev, "clava_sample_categories", _function("clava_sample_categories", "piliiipipplUUuppplp"),
+            logits.data_ptr(), dt, ld, B, m, sumk, op, max_classes, ctypes.byref(c), up, ld_u, seed & 0xFFFFFFFFFFFFFFFF,
+            row_offset & 0xFFFFFFFFFFFFFFFF, step_index & 0xFFFFFFFF, out.data_ptr(), None if lp is None else lp.data_ptr(),
+            None if ws is None else ws.data_ptr(), need)
     return (out, lp) if log_prob else out

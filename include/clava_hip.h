@@ -32,6 +32,7 @@ extern "C" {
 #define CLAVA_DT_F32 0
 #define CLAVA_DT_BF16 1
 #define CLAVA_DT_F16 2
+#define CLAVA_DT_MX4 3 /* microscaled 4-bit: codes and scales */
 
 int clava_version(void);
 const char* clava_last_error(void);
@@ -151,13 +152,17 @@ int clava_gemm_wgrad_f16x3_tn(const void* dy, long long pitch_dy, int shift_dy, 
  * clava_mx4_pack: scale exponent e = floor(log2(max |v|)) - 2 (clamped to -127 .. 127), code = nearest E2M1 of v / 2^e, ties to
  *   even, saturating at 6; a block that holds a NaN or an infinity gets scale 255 and reads as NaN.  src has row stride ld.
  * clava_mx4_unpack: dst[r * ld + c] = value(code) * 2^(scale - 127), rounded to `dtype`.
- * clava_linear_mx4: y[M,N] = act( x[M,K] . w[N,K]^T + bias[N] ), both operands as above, products summed in float32; the result
- *   as `y` (y_dtype, row stride ldy) or, with y == NULL, packed again as y_codes / y_scales (for the next layer).  codes
- *   pointers are 16-byte aligned.  dtype: CLAVA_DT_*; act: CLAVA_ACT_*_. */
+ * clava_linear_mx4: y[M,N] = act( x[M,K] . w[N,K]^T + bias[N] ), products summed in float32; w as above, x as above (x_dtype
+ *   CLAVA_DT_MX4: `x` its codes, x_scales) or a float matrix of row stride ldx, which is packed into `workspace` first
+ *   (clava_linear_mx4_workspace_bytes(M, K, x_dtype) bytes, 16-byte aligned).  The result as `y` (y_dtype, row stride ldy) or,
+ *   with y_dtype CLAVA_DT_MX4, packed again (`y` its codes, y_scales; for the next layer).  codes pointers are 16-byte
+ *   aligned.  dtype: CLAVA_DT_*; act: CLAVA_ACT_*_. */
 int clava_mx4_pack(const void* src, int dtype, long long ld, long long rows, int cols, void* codes, void* scales, void* stream);
 int clava_mx4_unpack(const void* codes, const void* scales, long long rows, int cols, void* dst, int dtype, long long ld, void* stream);
-int clava_linear_mx4(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, const float* bias, int act,
-                     void* y, int y_dtype, long long ldy, void* y_codes, void* y_scales, int M, int N, int K, void* stream);
+long long clava_linear_mx4_workspace_bytes(int M, int K, int x_dtype);
+int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_scales, const void* w_codes, const void* w_scales,
+                     const float* bias, int act, void* y, int y_dtype, long long ldy, void* y_scales, int M, int N, int K,
+                     void* workspace, void* stream);
 
 /* ---- schedule tables ---------------------------------------------------------------------------------------
  * Device-resident tables of length T, built by the host exactly as GaussianMultinomialDiffusion.__init__ builds
