@@ -1,7 +1,7 @@
 // Dense layer over microscaled 4-bit matrices: y[m][n] = act( sum over blocks of 2^(ex + ew) * (sum of 32 products of codes)
 // + bias[n] ).  v_mfma_scale_f32_16x16x128 takes both scales with the codes and accumulates in float32.  W is the instruction's
 // first operand, so that a lane ends up with neighbouring columns of one row of y.
-#include <cstdlib>
+#include <type_traits>
 
 #include "clava_hip.h"
 #include "mx4.h"
@@ -46,23 +46,31 @@ __device__ __forceinline__ void bias8(const Mx4Args& g, int n0, float* b) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) b[j] = 0.f;
 }
-// A lane's eight columns n0 .. n0+7 of row m (n0 a multiple of 8; lanes l, l^16, l^32, l^48 hold one block of 32 columns):
-// every lane of the wave calls this, also those outside of y.
-template <int OUT> __device__ __forceinline__ void finish(const Mx4Args& g, int m, int n0, const float* b, float* v) {
+// A lane's C = 8 or 16 columns n0 .. of row m (n0 a multiple of C).  The lanes that hold the rest of a block of 32 columns are
+// l^16, l^32, l^48 (C = 8) or l^32 (C = 16); every lane of the wave calls this, also those outside of y.
+template <int OUT, int C> __device__ __forceinline__ void finish(const Mx4Args& g, int m, int n0, const float* b, float* v) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += b[j];
-    activate8(v, g.act);
-    if (OUT != OUT_MX4) {
-        if (m < g.M && n0 < g.N) store8<OUT == OUT_MX4 ? 0 : OUT>(g.y, (size_t)m * g.ldy + n0, g.N - n0, v);
-        return;
+    for (int c = 0; c < C; c += 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[c + j] += b[c + j];
+        activate8(v + c, g.act);
+        if (OUT != OUT_MX4 && m < g.M && n0 + c < g.N) store8<OUT == OUT_MX4 ? 0 : OUT>(g.y, (size_t)m * g.ldy + n0 + c, g.N - n0 - c, v + c);
     }
+    if (OUT != OUT_MX4) return;
+    unsigned top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < C; ++j) {
         if (n0 + j >= g.N) v[j] = 0.f;
-    const int byte = scale_byte(block_max<16, 32>(v));
+        top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+    }
+    if (C == 8) top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
+    top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+    const int byte = scale_byte(top);
     if (m < g.M && n0 < g.yks * KSTEP) {
-        g.yq[((size_t)m * g.yks * KSTEP + n0) >> 3] = pack8(v, byte);
-        if ((n0 & 31) == 0) g.ys[((size_t)m * g.yks * KSTEP + n0) >> 5] = (unsigned char)byte;
+        const size_t at = (size_t)m * g.yks * KSTEP + n0;
+#pragma unroll
+        for (int c = 0; c < C; c += 8) g.yq[(at + c) >> 3] = pack8(v + c, byte);
+        if ((n0 & 31) == 0) g.ys[at >> 5] = (unsigned char)byte;
     }
 }
 
@@ -95,7 +103,7 @@ template <int OUT> __global__ void __launch_bounds__(256) mx4_linear_kernel(Mx4A
     float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     float bias[8];
     bias8(g, n0 + 8 * q, bias);
-    finish<OUT>(g, m0 + r, n0 + 8 * q, bias, v);
+    finish<OUT, 8>(g, m0 + r, n0 + 8 * q, bias, v);
 }
 
 
@@ -107,110 +115,165 @@ __device__ __forceinline__ void dma4(const void* src, char* dst) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
 }
 
-// BN columns x BM rows of y a workgroup of WN x WM wavefronts.  A stage is 256 columns of K: 128 bytes of codes a row (its
-// 16-byte chunks exchanged by row bits 1..3, so that the 16 rows of a fragment read hit different banks), then 8 bytes of
-// scales a row.  Two stages: the next one is copied straight to LDS while this one is multiplied.
-template <int BN, int BM, int WN, int WM, int OUT> __global__ void __launch_bounds__(WN * WM * 64) mx4_tile_kernel(Mx4Args g, int tiles_n, int tiles) {
-    constexpr int R = BN + BM, NW = WN * WM, Q = R / 8 / NW, QS = R / 32 / NW > 0 ? R / 32 / NW : 1, STAGE = R * 136;
-    constexpr int TN = BN / WN / 16, TM = BM / WM / 16;
-    static_assert(R % (8 * NW) == 0 && TN % 2 == 0 && (R / 32) % NW == 0, "tile");
+// BN columns x BM rows of y a workgroup of WN x WM wavefronts, on v_mfma_scale_f32_32x32x64: one wavefront a SIMD reaches
+// 9.0 PFLOP/s with it, and 3.3 with 16x16x128, whose scale load costs as much as its product (registers only, 256 workgroups).
+// A stage is 256 columns of K: 128 bytes of codes a row (its 16-byte chunks exchanged by row bits 1..3, so that the rows of a
+// fragment read hit different banks), NS of them in a ring.  Scales have a ring of their own.  S16: 16 bytes of them a row, 512
+// columns, in one copy (rows of whole 16 bytes: K a multiple of 512); else 4 bytes in each.  A copy of scales touches a cache
+// line per row, whatever it takes from it: with 4 bytes the scales took the copies of a 256 x 256 tile from 1.3 to 1.8 us a stage.
+template <int BN, int BM, int WN, int WM, int NS, bool S16, int OUT>
+__global__ void __launch_bounds__(WN * WM * 64) mx4_tile_kernel(Mx4Args g, int tiles_n, int tiles) {
+    constexpr int R = BN + BM, NW = WN * WM, Q = R / 8 / NW, STAGE = R * 128;
+    // copies of scales: of a group (S16: of two stages), of a wave; bytes of a row and of a group, groups in the ring
+    constexpr int SU = S16 ? R / 64 : R / 32, QS = (SU + NW - 1) / NW, SROW = S16 ? 16 : 8, SGROUP = R * SROW, SRING = S16 ? NS / 2 + 1 : NS;
+    constexpr int WAIT = (NS - 2) * Q + (S16 ? (NS - 2) / 2 : NS - 2) * QS;      // copies behind those of the stage that is next
+    constexpr int TN = BN / WN / 32, TM = BM / WM / 32;
+    static_assert(R % (8 * NW) == 0 && NW % 2 == 0 && NS % 2 == 0 && TN > 0 && TM > 0, "tile");
     extern __shared__ __align__(16) char smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wn = wave / WM, wm = wave % WM, r = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wn = wave / WM, wm = wave % WM, r = lane & 31, h = lane >> 5;
 
     // workgroups go round robin over the 8 XCDs: each takes a run of tiles, for its L2
     const int xcd = (int)blockIdx.x & 7, per = tiles >> 3, rem = tiles & 7;
     const int tile = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + ((int)blockIdx.x >> 3);
-    const int m0 = tile / tiles_n * BM, n0 = tile % tiles_n * BN;
+    // in it, eight tiles down before the next column: the 32 tiles that an XCD works on at a time then share 8 panels of X and 4
+    // of W (a row of tiles: 1 and 32)
+    const int tiles_m = tiles / tiles_n, group = tile / (8 * tiles_n), gm = min(8, tiles_m - 8 * group), in = tile - group * 8 * tiles_n;
+    const int m0 = (8 * group + in % gm) * BM, n0 = in / gm * BN;
 
-    // LDS row `row` of W holds the column of y that puts a lane's accumulators of two neighbouring tiles side by side
+    // LDS row `row` of W holds the column of y that puts the 16 accumulators of a lane side by side: its half h of a 32 x 32
+    // product has rows 8 G + 4 h + t, G, t < 4, and they are to be columns 16 h + 4 G + t.  Sources are a base of the tile (in scalar registers) and 32 bits of a lane's own.
+    const int nb = min(n0, g.N - 1);
+    const char *wq = g.wq + (size_t)nb * g.ks * 64, *xq = g.xq + (size_t)m0 * g.ks * 64;
+    const unsigned char *ws = g.ws + (size_t)nb * g.ks * 4, *xs = g.xs + (size_t)m0 * g.ks * 4;
     auto source_row = [&](int row) {
-        if (row >= BN) return (size_t)min(m0 + row - BN, g.M - 1);
-        return (size_t)min(n0 + (row & ~31) + pair_row(row & 15, row >> 4 & 1), g.N - 1);
+        if (row >= BN) return (unsigned)(min(m0 + row - BN, g.M - 1) - m0);
+        return (unsigned)(min(n0 + (row & ~31) + 16 * (row >> 2 & 1) + 4 * (row >> 3 & 3) + (row & 3), g.N - 1) - nb);
     };
-    const char* src[Q];
-    int half[Q];
+    unsigned src[Q], ssrc[QS];
 #pragma unroll
     for (int j = 0; j < Q; ++j) {
         const int row = (wave + j * NW) * 8 + (lane >> 3), chunk = (lane & 7) ^ (row >> 1 & 7);
-        src[j] = (row < BN ? g.wq : g.xq) + source_row(row) * g.ks * 64 + (chunk & 3) * 16;
-        half[j] = chunk >> 2;
+        src[j] = source_row(row) * (unsigned)g.ks * 64u + (unsigned)chunk * 16u;
     }
-    const unsigned char* ssrc[QS];
 #pragma unroll
     for (int j = 0; j < QS; ++j) {
-        const int row = (wave + j * NW) * 32 + (lane >> 1);
-        ssrc[j] = (row < BN ? g.ws : g.xs) + source_row(row) * g.ks * 4;
+        const int u = min(wave + j * NW, SU - 1);
+        ssrc[j] = S16 ? source_row(u * 64 + lane) * (unsigned)g.ks * 4u : source_row(u * 32 + (lane >> 1)) * (unsigned)g.ks * 4u + (unsigned)(lane & 1) * 4u;
     }
+    char* const scales = smem + NS * STAGE;
     const int stages = (g.ks + 1) >> 1;
+    // (an odd number of steps: the second half of the last stage is a copy of the first, and not multiplied.  Which half a lane
+    // copies does not depend on j: NW * 8 rows are a multiple of 16.)
+    const unsigned second = (unsigned)((lane & 7) ^ ((wave * 8 + (lane >> 3)) >> 1 & 7)) >> 2;
+    // Stage s, or behind the end the last one again (to where nobody reads), so that every wave always has the same number of
+    // copies under way
     auto copy = [&](int s, char* to) {
-        // an odd number of steps: the second half of the last stage is a copy of the first, and not multiplied
-        const bool whole = 2 * s + 1 < g.ks;
+        const int d = min(s, stages - 1);
+        const bool whole = 2 * d + 1 < g.ks;
+        const char *w = wq + (size_t)d * 128, *x = xq + (size_t)d * 128;
 #pragma unroll
-        for (int j = 0; j < Q; ++j) dma16(src[j] + (2 * s + (whole ? half[j] : 0)) * 64, to + (wave + j * NW) * 1024);
+        for (int j = 0; j < Q; ++j) dma16(((wave + j * NW) * 8 < BN ? w : x) + (S16 || whole ? src[j] : src[j] - second * 64u), to + (wave + j * NW) * 1024);
+        if (S16 && (s & 1)) return;
+        const unsigned char *sw = ws + (size_t)(S16 ? d >> 1 : d) * SROW, *sx = xs + (size_t)(S16 ? d >> 1 : d) * SROW;
+        char* const ring = scales + (S16 ? s >> 1 : s) % SRING * SGROUP;
 #pragma unroll
-        for (int j = 0; j < QS; ++j)
-            dma4(ssrc[j] + (2 * s + (whole ? lane & 1 : 0)) * 4, to + R * 128 + (wave + j * NW) * 256);
+        for (int j = 0; j < QS; ++j) {
+            const int u = min(wave + j * NW, SU - 1);
+            if (S16) dma16((u * 64 < BN ? sw : sx) + ssrc[j], ring + u * 1024);
+            else dma4((u * 32 < BN ? sw : sx) + (whole ? ssrc[j] : ssrc[j] - (unsigned)(lane & 1) * 4u), ring + u * 256);
+        }
     };
 
-    const int frag = r * 128, swz = r >> 1 & 7;
-    const int wrow = wn * TN * 16, xrow = BN + wm * TM * 16;
-    f32x4 acc[TN][TM];
+    const int wrow = wn * TN * 32, xrow = BN + wm * TM * 32, swz = r >> 1 & 7;
+    f32x16 acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.f;
 
-    auto step = [&](const char* at, int ks) {
-        const int off = frag + (((ks * 4 + q) ^ swz) << 4);
-        const char* sc = at + R * 128 + r * 8 + ks * 4;
-        i32x8 X[TM];
-        int sx[TM];
+    // One stage: STEPS (4, or 2 of a half one) steps of 64 columns, each TN groups of TM products.  W is read two groups ahead,
+    // the next step's X one step ahead, so that a product does not wait for the read before it.
+    auto multiply = [&](const char* at, int s, auto steps_t) {
+        constexpr int STEPS = decltype(steps_t)::value, GROUPS = STEPS * TN;
+        const char *w = at + (wrow + r) * 128, *x = at + (xrow + r) * 128;
+        const char* const es_at = scales + (S16 ? s >> 1 : s) % SRING * SGROUP + (S16 ? (s & 1) * 8 : 0) + r * SROW;
+        i32x4 X[2][TM], W[3];
+        auto read_w = [&](int grp) { return *reinterpret_cast<const i32x4*>(w + (((grp / TN * 2 + h) ^ swz) << 4) + (grp % TN) * 4096); };
+        auto read_x = [&](int ks, int j) { return *reinterpret_cast<const i32x4*>(x + (((ks * 2 + h) ^ swz) << 4) + j * 4096); };
+        u32x2 es[TN], ex[TM];
 #pragma unroll
-        for (int j = 0; j < TM; ++j) {
-            const i32x4 v = *reinterpret_cast<const i32x4*>(at + (xrow + j * 16) * 128 + off);
-            X[j] = i32x8{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
-            sx[j] = (int)(*reinterpret_cast<const unsigned*>(sc + (xrow + j * 16) * 8) >> (8 * q));
-        }
+        for (int j = 0; j < TM; ++j) ex[j] = *reinterpret_cast<const u32x2*>(es_at + (xrow + j * 32) * SROW);
 #pragma unroll
-        for (int i = 0; i < TN; ++i) {
-            const i32x4 v = *reinterpret_cast<const i32x4*>(at + (wrow + i * 16) * 128 + off);
-            const i32x8 W = {v[0], v[1], v[2], v[3], 0, 0, 0, 0};
-            const int sw = (int)(*reinterpret_cast<const unsigned*>(sc + (wrow + i * 16) * 8) >> (8 * q));
+        for (int i = 0; i < TN; ++i) es[i] = *reinterpret_cast<const u32x2*>(es_at + (wrow + i * 32) * SROW);
+        W[0] = read_w(0);
 #pragma unroll
-            for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(W, X[j], acc[i][j], 4, 4, 0, sw, 0, sx[j]);
+        for (int j = 0; j < TM; ++j) X[0][j] = read_x(0, j);
+        W[1] = read_w(1);
+        // a lane's bytes of a dword are those of its half of two steps: bits 0 and 16 after the shift
+#pragma unroll
+        for (int j = 0; j < TM; ++j) ex[j] = ex[j] >> (unsigned)(8 * h);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) es[i] = es[i] >> (unsigned)(8 * h);
+#pragma unroll
+        for (int grp = 0; grp < GROUPS; ++grp) {
+            const int ks = grp / TN, i = grp % TN;
+            if (grp + 2 < GROUPS) W[(grp + 2) % 3] = read_w(grp + 2);
+            if (i == 0 && ks + 1 < STEPS)
+#pragma unroll
+                for (int j = 0; j < TM; ++j) X[(ks + 1) & 1][j] = read_x(ks + 1, j);
+            const i32x4 v = W[grp % 3];
+            const i32x8 A = {v[0], v[1], v[2], v[3], 0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+                const i32x4 u = X[ks & 1][j];
+                const i32x8 B = {u[0], u[1], u[2], u[3], 0, 0, 0, 0};
+                if (ks & 1) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, acc[i][j], 4, 4, 2, (int)es[i][ks >> 1], 2, (int)ex[j][ks >> 1]);
+                else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, acc[i][j], 4, 4, 0, (int)es[i][ks >> 1], 0, (int)ex[j][ks >> 1]);
+            }
         }
     };
-    copy(0, smem);
-    int cur = 0;
-    for (int s = 0; s < stages; ++s) {
-        __syncthreads();          // stage s has landed, and nobody reads the other one any more
-        if (s + 1 < stages) copy(s + 1, smem + (STAGE - cur));
-        step(smem + cur, 0);
-        if (2 * s + 1 < g.ks) step(smem + cur, 1);
-        cur = STAGE - cur;
-    }
+    // Stages s + 1 .. s + NS - 1 are on their way while stage s is multiplied; the counted wait says that stage s is there
 #pragma unroll
-    for (int i = 0; i < TN; i += 2) {
-        const int n = n0 + (wn * TN + i) * 16 + 8 * q;
-        float bias[8];
+    for (int s = 0; s < NS - 1; ++s) copy(s, smem + s * STAGE);
+    int cur = 0, nxt = (NS - 1) * STAGE;
+    for (int s = 0; s < g.ks >> 1; ++s) {
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WAIT) : "memory");
+        copy(s + NS - 1, smem + nxt);
+        multiply(smem + cur, s, std::integral_constant<int, 4>{});
+        nxt = cur;
+        cur = cur + STAGE == NS * STAGE ? 0 : cur + STAGE;
+    }
+    if (!S16 && (g.ks & 1)) {
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WAIT) : "memory");
+        multiply(smem + cur, stages - 1, std::integral_constant<int, 2>{});
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the last copies land before the LDS is someone else's
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+        const int n = n0 + (wn * TN + i) * 32 + 16 * h;
+        float bias[16];
         bias8(g, n, bias);
+        bias8(g, n + 8, bias + 8);
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
-            float v[8] = {acc[i][j][0],     acc[i][j][1],     acc[i][j][2],     acc[i][j][3],
-                          acc[i + 1][j][0], acc[i + 1][j][1], acc[i + 1][j][2], acc[i + 1][j][3]};
-            finish<OUT>(g, m0 + (wm * TM + j) * 16 + r, n, bias, v);
+            float v[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = acc[i][j][k];
+            finish<OUT, 16>(g, m0 + (wm * TM + j) * 32 + r, n, bias, v);
         }
     }
 }
 
-template <int BN, int BM, int WN, int WM, int OUT> int launch_tile(const Mx4Args& g, int n_cols, hipStream_t st) {
-    constexpr int LDS = (BN + BM) * 136 * 2;
+template <int BN, int BM, int WN, int WM, int NS, bool S16, int OUT> int launch_tile_s(const Mx4Args& g, int n_cols, hipStream_t st) {
+    constexpr int LDS = (BN + BM) * (128 * NS + (S16 ? 16 * (NS / 2 + 1) : 8 * NS));
     static bool set[64] = {};     // by device (threads that race set the same value twice)
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
     if (!set[dev]) {
-        if (hipFuncSetAttribute((const void*)mx4_tile_kernel<BN, BM, WN, WM, OUT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
+        if (hipFuncSetAttribute((const void*)mx4_tile_kernel<BN, BM, WN, WM, NS, S16, OUT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
             clava_set_error("linear_mx4: %d bytes of LDS refused", LDS);
             return CLAVA_ERR_LAUNCH;
         }
@@ -222,21 +285,28 @@ template <int BN, int BM, int WN, int WM, int OUT> int launch_tile(const Mx4Args
         clava_set_error("linear_mx4: %d x %d outputs are more than one launch takes", g.M, g.N);
         return CLAVA_ERR_LIMIT;
     }
-    mx4_tile_kernel<BN, BM, WN, WM, OUT><<<dim3((unsigned)tiles), WN * WM * 64, LDS, st>>>(g, tiles_n, (int)tiles);
+    mx4_tile_kernel<BN, BM, WN, WM, NS, S16, OUT><<<dim3((unsigned)tiles), WN * WM * 64, LDS, st>>>(g, tiles_n, (int)tiles);
     return CLAVA_OK;
+}
+
+template <int BN, int BM, int WN, int WM, int NS, int OUT> int launch_tile(const Mx4Args& g, int n_cols, hipStream_t st) {
+    if (g.ks % 4 == 0 && (((uintptr_t)g.xs | (uintptr_t)g.ws) & 15) == 0) return launch_tile_s<BN, BM, WN, WM, NS, true, OUT>(g, n_cols, st);
+    return launch_tile_s<BN, BM, WN, WM, NS, false, OUT>(g, n_cols, st);
 }
 
 template <int OUT> int launch_linear(const Mx4Args& g, hipStream_t st) {
     // a 4-bit result also has the zero codes behind its last column written: its columns go to the whole step
     const int n_cols = OUT == OUT_MX4 ? g.yks * KSTEP : g.N;
     const int tiles_n = (n_cols + 31) / 32;
-    static const char* force = getenv("CLAVA_MX4_TILE");
-    const int f = force ? atoi(force) : 0;
-    if (f == 1 || (f == 0 && g.M > 64)) {
-        if (f == 0 && (long long)((g.M + 255) / 256) * ((n_cols + 255) / 256) >= 256) return launch_tile<256, 256, 2, 4, OUT>(g, n_cols, st);
-        return launch_tile<128, 128, 2, 2, OUT>(g, n_cols, st);
+    // Many rows: the largest tile that still gives every CU two rounds of work (a large tile copies least per product; us for
+    // 256 x 256 / 128 x 128 / 64 x 64 tiles: 16384 x 8192 x 8192 591 / 672 / 1056, 20000 x 1024 x 1024 28.6 / 22.8 / 38.8,
+    // 4096 x 1024 x 1024 14.3 / 7.7 / 10.1, 1024 x 1024 x 1024 13.4 / 6.2 / 4.7, 256 x 4096 x 4096 30.6 / 12.9 / 8.5).
+    auto tiles = [&](int t) { return (long long)((g.M + t - 1) / t) * ((n_cols + t - 1) / t); };
+    if (g.M > 64) {
+        if (tiles(256) >= 512) return launch_tile<256, 256, 2, 4, 2, OUT>(g, n_cols, st);
+        if (tiles(128) >= 256) return launch_tile<128, 128, 2, 4, 2, OUT>(g, n_cols, st);
+        return launch_tile<64, 64, 2, 2, 4, OUT>(g, n_cols, st);
     }
-    if (f == 2) return launch_tile<256, 256, 2, 4, OUT>(g, n_cols, st);
     const long long wgs = (long long)((g.M + 15) / 16) * tiles_n;
     if (wgs > 0x7fffffffLL) {
         clava_set_error("linear_mx4: %d x %d outputs are more than one launch takes", g.M, g.N);

@@ -34,6 +34,8 @@ __device__ __forceinline__ unsigned pack8(const float* v, int byte) {
 }
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // Largest magnitude (as bits) of the 8 values of this lane and of the three lanes that hold the rest of its block, which
