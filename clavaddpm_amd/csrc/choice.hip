@@ -20,38 +20,59 @@ namespace {
 using namespace elem;
 typedef unsigned long long u64;
 
+constexpr double LOG2E = 1.44269504088896340736, LN2 = 0.69314718055994530942;
+
+// The parameters of a draw, ready to use
+struct Params {
+    double c, top_p, min_p;                   // log2(e) / T; in (0, 1], 1: off; in [0, 1]
+    float T;                                  // for bin widths only
+    int top_k;                                // 0: off
+    bool bad;                                 // the temperature is negative or no number
+};
+__host__ __device__ __forceinline__ Params params_of(double T, double top_p, double min_p, int top_k) {
+    Params p;
+    p.bad = !(T >= 0.0);
+    if (!(T >= 1e-290)) { T = 1.0; top_k = 1; }              // 0, and what 1 / T has no float64 for
+    p.c = LOG2E / T;
+    if (p.c < 1e-290) p.c = 1e-290;                          // (an infinite T: -inf * c stays -inf)
+    p.T = T < 1e30 ? (float)T : 1e30f;
+    p.top_k = top_k > 0 ? top_k : 0;
+    p.min_p = min_p > 0.0 ? (min_p < 1.0 ? min_p : 1.0) : 0.0;
+    p.top_p = top_p < 1.0 ? (top_p > 1e-290 ? top_p : 1e-290) : 1.0;       // the first of the order always stays; NaN: off
+    return p;
+}
+
 struct Choice {
     const void* z; long long ld;
     int B, m, sumK;
     const int* offsets;
     clava_choice p;
-    double c;                                 // log2(e) / temperature, where that is one number
+    Params same;                              // for all blocks, unless one of them is a tensor
+    bool tensors;
     const float* u; long long ld_u;
     unsigned long long seed, row_offset;
     unsigned step;
     int* idx; float* log_prob;
-    int wide_from;                            // blocks with more classes belong to the wide_* kernels; 0: there are none
+    bool wide;                                // blocks with more than wide_from classes belong to the wide_* kernels
+    int wide_from;
 };
 
-constexpr double LOG2E = 1.44269504088896340736, LN2 = 0.69314718055994530942;
-
-// 2^y for y <= 0: n = rint(y), 2^(y - n) by its power series (12 terms: (ln2/2)^13 / 13! < 2e-16), scaled by 2^n.
+// 2^y for y <= 0 (NaN and what is below float64: 0): n = rint(y), 2^(y - n) by its power series in base 2, ln2^k / k!, up to
+// k = 11 (the next term is 6e-15 at |y - n| = 1/2), scaled by 2^n.
+struct Exp2Terms {
+    double t[12];
+    constexpr Exp2Terms() : t{} {
+        t[0] = 1.0;
+        for (int k = 1; k < 12; ++k) t[k] = t[k - 1] * LN2 / k;
+    }
+};
 __device__ __forceinline__ double exp2_nonpos(double y) {
-    y = fmax(y, -1100.0);                     // below float64's smallest subnormal
-    const double n = rint(y), r = (y - n) * LN2;
-    double p = 1.0 / 479001600;
-    p = fma(p, r, 1.0 / 39916800);
-    p = fma(p, r, 1.0 / 3628800);
-    p = fma(p, r, 1.0 / 362880);
-    p = fma(p, r, 1.0 / 40320);
-    p = fma(p, r, 1.0 / 5040);
-    p = fma(p, r, 1.0 / 720);
-    p = fma(p, r, 1.0 / 120);
-    p = fma(p, r, 1.0 / 24);
-    p = fma(p, r, 1.0 / 6);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
+    constexpr Exp2Terms c;
+    y = fmax(y, -1100.0);
+    const double n = rint(y), r = y - n;
+    double p = c.t[11];
+#pragma unroll
+    for (int k = 10; k >= 0; --k) p = fma(p, r, c.t[k]);
     return ldexp(p, (int)n);
 }
 // log(x) for x >= 1: the float32 logarithm and one Newton step on e^y = x (its square, 1e-14, is what stays)
@@ -67,15 +88,6 @@ __device__ __forceinline__ unsigned key_of(float z) {
 // Position in the order: larger comes first; equal keys by index
 __device__ __forceinline__ u64 place_of(unsigned key, unsigned index) { return (u64)key << 32 | (unsigned)~index; }
 
-// A block and its parameters, ready to use.
-struct Block {
-    int b, f, K;
-    size_t at;
-    double u, c, top_p, min_p;                // top_p in (0, 1], 1: off; min_p in [0, 1]
-    float T;                                  // for bin widths only
-    int top_k;                                // 0: off
-    bool bad;                                 // a parameter or u is not a number
-};
 __device__ __forceinline__ int first_of(const Choice& g, int f) { return g.offsets ? max(0, min(g.offsets[f], g.sumK)) : 0; }
 __device__ __forceinline__ int classes_of(const Choice& g, int f) {
     return g.offsets ? max(0, min(g.offsets[f + 1], g.sumK) - first_of(g, f)) : g.sumK;
@@ -85,35 +97,33 @@ __device__ __forceinline__ double uniform_of(const Choice& g, int b, int f) {
     const unsigned long long e = (g.row_offset + (unsigned long long)b) * (unsigned long long)g.m + (unsigned long long)f;
     return (double)clava_rng::to_uniform(clava_rng::philox4x32_10(g.seed, e, g.step, clava_rng::STREAM_CHOICE).x);
 }
+// A block, its parameters and random number
+struct Block : Params {
+    int b, f, K;
+    size_t at;
+    double u;
+};
 __device__ __forceinline__ Block block_of(const Choice& g, int b, int f, int k0, int K) {
     Block x;
+    static_cast<Params&>(x) = g.same;
+    if (g.tensors) {
+        const clava_choice& p = g.p;
+        const double T = p.temperature_t ? (double)p.temperature_t[b * p.temperature_rs + f * p.temperature_fs] : p.temperature;
+        const double top_p = p.top_p_t ? (double)p.top_p_t[b * p.top_p_rs + f * p.top_p_fs] : p.top_p;
+        const double min_p = p.min_p_t ? (double)p.min_p_t[b * p.min_p_rs + f * p.min_p_fs] : p.min_p;
+        static_cast<Params&>(x) = params_of(T, top_p, min_p, p.top_k_t ? p.top_k_t[b * p.top_k_rs + f * p.top_k_fs] : p.top_k);
+    }
     x.b = b; x.f = f; x.K = K;
     x.at = (size_t)b * g.ld + k0;
     x.u = uniform_of(g, b, f);
-    const clava_choice& p = g.p;
-    double T = p.temperature;
-    x.c = g.c;
-    if (p.temperature_t) {
-        T = (double)p.temperature_t[b * p.temperature_rs + f * p.temperature_fs];
-        x.c = LOG2E / T;
-    }
-    x.top_p = p.top_p_t ? (double)p.top_p_t[b * p.top_p_rs + f * p.top_p_fs] : p.top_p;
-    x.min_p = p.min_p_t ? (double)p.min_p_t[b * p.min_p_rs + f * p.min_p_fs] : p.min_p;
-    x.top_k = p.top_k_t ? p.top_k_t[b * p.top_k_rs + f * p.top_k_fs] : p.top_k;
-    x.bad = x.u != x.u || !(T >= 0.0);
+    x.bad |= x.u != x.u;
     x.u = fmax(x.u, 0.0);
-    if (T < 1e-290) { x.c = LOG2E; T = 1.0; x.top_k = 1; }   // 0, and what 1 / T has no float64 for
-    x.T = (float)fmin(T, 1e30);
-    if (x.top_k < 0) x.top_k = 0;
-    x.min_p = fmin(fmax(x.min_p, 0.0), 1.0);                 // (fmax of a NaN: 0)
-    x.top_p = x.top_p < 1.0 ? fmax(x.top_p, 1e-290) : 1.0;   // the first of the order always stays; NaN: off
     return x;
 }
-// log2 of a class's mass, and the mass; +inf logits, where there are any, share the mass
-__device__ __forceinline__ double log2_mass(float z, float top, double c) {
-    if (top == INFINITY) return z == INFINITY ? 0.0 : -INFINITY;
-    return z == -INFINITY ? -INFINITY : ((double)z - (double)top) * c;
-}
+// +inf logits, where there are any, share the mass: as zeros among -inf
+__device__ __forceinline__ float settle(float z, bool inf) { return inf ? (z == INFINITY ? 0.f : -INFINITY) : z; }
+// log2 of a class's mass, and the mass, from its logit and the largest one, which is finite (-inf: no mass)
+__device__ __forceinline__ double log2_mass(float z, float top, double c) { return ((double)z - (double)top) * c; }
 __device__ __forceinline__ double mass_of(float z, float top, double c) { return exp2_nonpos(log2_mass(z, top, c)); }
 // a in units of 2^-s, s <= 51, to the nearest: the fraction bits of a * 2^s + 2^52
 __device__ __forceinline__ u64 units(double a, double scale) {
@@ -182,9 +192,24 @@ __device__ __forceinline__ u64 from_lane(u64 v, int lane) {
 __device__ __forceinline__ double from_lane(double v, int lane) {
     return __longlong_as_double((long long)from_lane((u64)__double_as_longlong(v), lane));
 }
-__device__ __forceinline__ u64 from_xor(u64 v, int mask) {
-    return (u64)(unsigned)__shfl_xor((int)(v >> 32), mask, 64) << 32 | (unsigned)__shfl_xor((int)v, mask, 64);
+// The same for a lane that is the same in the whole wavefront, without a way through LDS
+__device__ __forceinline__ int at_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ u64 at_lane(u64 v, int lane) { return (u64)(unsigned)at_lane((int)(v >> 32), lane) << 32 | (unsigned)at_lane((int)v, lane); }
+__device__ __forceinline__ double at_lane(double v, int lane) {
+    return __longlong_as_double((long long)at_lane((u64)__double_as_longlong(v), lane));
 }
+// Lane l's value of lane l ^ d: moves within rows of 16 lanes, exchanges of rows and halves
+__device__ __forceinline__ int from_xor(int v, int d) {
+    constexpr int QUAD_MIRROR = 0x1B;
+    if (d == 1) return dpp_i<DPP_XOR1>(v);
+    if (d == 2) return dpp_i<DPP_XOR2>(v);
+    if (d == 4) return dpp_i<QUAD_MIRROR>(dpp_i<DPP_HALF_MIRROR>(v));            // l ^ 7 ^ 3
+    if (d == 8) return dpp_i<DPP_HALF_MIRROR>(dpp_i<DPP_ROW_MIRROR>(v));         // l ^ 15 ^ 7
+    const auto o = d == 16 ? __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false)
+                           : __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+    return (int)(lane_here() & d ? o[0] : o[1]);
+}
+__device__ __forceinline__ u64 from_xor(u64 v, int d) { return (u64)(unsigned)from_xor((int)(v >> 32), d) << 32 | (unsigned)from_xor((int)v, d); }
 // Bitonic sort within groups of G lanes, largest first
 template <int G> __device__ __forceinline__ u64 sort_falling(u64 v) {
     const int l = lane_here() & (G - 1);
@@ -199,13 +224,38 @@ template <int G> __device__ __forceinline__ u64 sort_falling(u64 v) {
     return v;
 }
 
+// What a wavefront has chosen, a block a lane: the logarithms and the stores of 64 blocks are done together
+struct Chosen {
+    unsigned n, out;
+    int index;
+    double y, total;
+    __device__ __forceinline__ void flush(const Choice& g) {
+        if ((threadIdx.x & 63) < n) {
+            g.idx[out] = index;
+            if (g.log_prob) g.log_prob[out] = (float)(y * LN2 - log_from1(total));
+        }
+        n = 0;
+    }
+    __device__ __forceinline__ void add(const Choice& g, const Block& x, int i, double log2_a, double mass) {
+        if ((threadIdx.x & 63) == n) {
+            out = (unsigned)x.b * (unsigned)g.m + (unsigned)x.f;
+            index = i;
+            y = log2_a;
+            total = mass;
+        }
+        if (++n == 64) flush(g);
+    }
+};
+
 // The whole choice among the classes that a group's lanes hold, one each, in index order: `z` (-inf and key 0 where a lane holds
 // none), their index, the block's maximum.  `nan`: the block holds a NaN.  All lanes of the wave come here together.
 template <int G> __device__ __forceinline__ void choose_lanes(const Choice& g, const Block& x, float z, unsigned key, int index, float top,
-                                                              bool nan, bool live) {
+                                                              bool nan, bool live, Chosen* chosen) {
     const int lane = threadIdx.x & 63, base = lane & ~(G - 1), l = lane & (G - 1);
-    const u64 group = (G == 64 ? ~0ull : ((1ull << G) - 1)) << base;
-    const double y = log2_mass(z, top, x.c), a = exp2_nonpos(y);
+    const u64 group = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1)) << base;
+    auto last_of = [&](auto v) { return G == 64 ? at_lane(v, 63) : from_lane(v, base + G - 1); };
+    const bool inf = top == INFINITY;
+    const double y = log2_mass(settle(z, inf), inf ? 0.f : top, x.c), a = exp2_nonpos(y);
     bool keep = a >= x.min_p;
     if (__any(x.top_k > 0 || x.top_p < 1.0)) {
         const u64 place = (u64)key << 32 | (unsigned)(63 - lane);
@@ -213,20 +263,26 @@ template <int G> __device__ __forceinline__ void choose_lanes(const Choice& g, c
         const bool in = x.top_k == 0 || l < x.top_k;
         const double as = from_lane(a, 63 - (int)(unsigned)sorted);
         const double w = in ? as : 0.0, run = scan<G>(w);
-        const double goal = x.top_p * from_lane(run, base + G - 1);
+        const double goal = x.top_p * last_of(run);
         const bool stay = in && (l == 0 || x.top_p >= 1.0 || run - w < goal);
         const u64 out = ~(__ballot(stay) >> base) | (G == 64 ? 0 : 1ull << (G & 63));
         const int n = out ? (int)__builtin_ctzll(out) : 64;      // those before the first that goes
-        const u64 last = from_lane(sorted, base + n - 1);        // (every lane gives its own: not behind a lane's condition)
+        const u64 last = G == 64 ? at_lane(sorted, n - 1) : from_lane(sorted, base + n - 1);      // (of every lane: not behind `keep`)
         keep = keep && place >= last;
     }
-    const double w = keep ? a : 0.0, run = scan<G>(w), total = from_lane(run, base + G - 1);
+    const double w = keep ? a : 0.0, run = scan<G>(w), total = last_of(run);
     const double goal = x.u * total;
     const u64 can = __ballot(w > 0.0) & group, past = __ballot(w > 0.0 && run > goal) & group;
-    if (!live) return;
     const bool none = nan || x.bad || top == -INFINITY;
     const int hit = past ? (int)__builtin_ctzll(past) : can ? 63 - (int)__builtin_clzll(can) : 0;
-    if (none ? l == 0 : lane == hit) give(g, x.b, x.f, none ? -1 : index, none ? no_number() : (float)(y * LN2 - log_from1(total)));
+    if (G == 64) {
+        if (none) {
+            if (lane == 0) give(g, x.b, x.f, -1, no_number());
+        } else chosen->add(g, x, at_lane(index, hit), at_lane(y, hit), total);
+    } else {
+        const float lp = g.log_prob ? (float)(y * LN2 - log_from1(total)) : 0.f;
+        if (live && (none ? l == 0 : lane == hit)) give(g, x.b, x.f, none ? -1 : index, none ? no_number() : lp);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------- a wavefront's block
@@ -293,7 +349,7 @@ __device__ __forceinline__ u64 find_edge(const WaveBlock& w, u64 bins, double go
         const u64 run = scan<64>(bins), past = __ballot((double)(before + run) >= goal);
         if (past == 0) return 0;
         const int at = (int)__builtin_ctzll(past);
-        before += from_lane(run - bins, at);
+        before += at_lane(run - bins, at);
         // the classes of that bin
         int count = 0;
         unsigned klo = 0xffffffffu, khi = 0;
@@ -320,7 +376,7 @@ __device__ __forceinline__ u64 find_edge(const WaveBlock& w, u64 bins, double go
             const int pos = 63 - (int)(sorted & 63);
             const u64 sum = scan<64>(lane < count ? s.weight[pos] : (u64)0);
             const u64 there = __ballot(lane < count && (double)(before + sum) >= goal);
-            return from_lane(mine, __shfl(pos, there ? (int)__builtin_ctzll(there) : count - 1, 64));
+            return at_lane(mine, at_lane(pos, there ? (int)__builtin_ctzll(there) : count - 1));
         }
         lo = wave_min(klo);
         hi = wave_max(khi);
@@ -352,76 +408,88 @@ __device__ __forceinline__ u64 find_edge(const WaveBlock& w, u64 bins, double go
     }
 }
 
-// Sums over the wave of four values at once: halves, then rows of 16 change places, so that row r ends up with value r
-__device__ __forceinline__ void swap32(double& a, double& b) {
+// Sums over the wave of four values at once: halves, then rows of 16 change places, so that the lanes of row r get value r's
+__device__ __forceinline__ void swap_halves(double& a, double& b) {
     const u64 p = (u64)__double_as_longlong(a), q = (u64)__double_as_longlong(b);
     const auto lo = __builtin_amdgcn_permlane32_swap((unsigned)p, (unsigned)q, false, false);
     const auto hi = __builtin_amdgcn_permlane32_swap((unsigned)(p >> 32), (unsigned)(q >> 32), false, false);
     a = __longlong_as_double((long long)((u64)hi[0] << 32 | lo[0]));
     b = __longlong_as_double((long long)((u64)hi[1] << 32 | lo[1]));
 }
-__device__ __forceinline__ void swap16(double& a, double& b) {
+__device__ __forceinline__ void swap_rows(double& a, double& b) {
     const u64 p = (u64)__double_as_longlong(a), q = (u64)__double_as_longlong(b);
     const auto lo = __builtin_amdgcn_permlane16_swap((unsigned)p, (unsigned)q, false, false);
     const auto hi = __builtin_amdgcn_permlane16_swap((unsigned)(p >> 32), (unsigned)(q >> 32), false, false);
     a = __longlong_as_double((long long)((u64)hi[0] << 32 | lo[0]));
     b = __longlong_as_double((long long)((u64)hi[1] << 32 | lo[1]));
 }
-__device__ __forceinline__ double lane_value(double v, int lane) {
-    const u64 b = (u64)__double_as_longlong(v);
-    return __longlong_as_double((long long)((u64)(unsigned)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 |
-                                            (unsigned)__builtin_amdgcn_readlane((int)b, lane)));
-}
-__device__ __forceinline__ void sums4(double (&v)[4]) {
-    swap32(v[0], v[2]);
-    swap32(v[1], v[3]);
-    double a = v[0] + v[2], b = v[1] + v[3];
-    swap16(a, b);
+__device__ __forceinline__ double row_sums(double v0, double v1, double v2, double v3) {
+    swap_halves(v0, v2);
+    swap_halves(v1, v3);
+    double a = v0 + v2, b = v1 + v3;
+    swap_rows(a, b);
     a += b;
     a += dpp_d<DPP_XOR1>(a);
     a += dpp_d<DPP_XOR2>(a);
     a += dpp_d<DPP_HALF_MIRROR>(a);
-    a += dpp_d<DPP_ROW_MIRROR>(a);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = lane_value(a, 16 * r);
+    return a + dpp_d<DPP_ROW_MIRROR>(a);
 }
 
 // A block of up to 64 * (floats of zs / 64) classes.  Its logits stay in LDS: the passes over them are loops of a run-time
 // length then, and the compiler keeps no register per slot (with the block in registers the unrolled passes took 232 of them
 // and two wavefronts a SIMD).
-template <int DT> __device__ __forceinline__ void choose_wave(const Choice& g, const Block& x, float* zs, WaveLds& s) {
+template <int DT> __device__ __forceinline__ void choose_wave(const Choice& g, const Block& x, float* zs, WaveLds& s, Chosen& chosen) {
     const int lane = threadIdx.x & 63;
+    const bool cut_k = x.top_k > 0 && x.top_k < x.K, cut_p = x.top_p < 1.0;
     WaveBlock w;
     w.z = zs;
     w.n = (x.K + 63) >> 6;
-    float top = -INFINITY, bottom = INFINITY;
-    bool nan = false;
+    float top = -INFINITY;
+    unsigned largest = 0;                                    // magnitude, as bits: above infinity's for a NaN
     lds_order();
-#pragma unroll 4
-    for (int j = 0; j < w.n; ++j) {
-        const int i = j * 64 + lane;
-        const float z = i < x.K ? load1<DT>(g.z, x.at + i) : -INFINITY;
-        nan |= z != z;
+    auto take = [&](int j, float z) {
+        largest = max(largest, __float_as_uint(z) & 0x7fffffffu);
         top = fmaxf(top, z);
-        bottom = z == -INFINITY ? bottom : fminf(bottom, z);
+        zs[j * 64 + lane] = z;
+    };
+#pragma unroll 4
+    for (int j = 0; j < x.K >> 6; ++j) take(j, load1<DT>(g.z, x.at + j * 64 + lane));
+    if (x.K & 63) {
+        const int i = (x.K & ~63) + lane;
+        float z = -INFINITY;
+        if (i < x.K) z = load1<DT>(g.z, x.at + i);
+        top = fmaxf(top, z);
+        if (i < x.K) largest = max(largest, __float_as_uint(z) & 0x7fffffffu);
         zs[i] = z;
     }
     lds_order();
     top = group_max<64>(top);
-    if (__any(nan) || x.bad || top == -INFINITY) {
+    if (__any(largest > 0x7f800000u) || x.bad || top == -INFINITY) {
         if (lane == 0) give(g, x.b, x.f, -1, no_number());
         return;
     }
-    const bool cut_k = x.top_k > 0 && x.top_k < x.K, cut_p = x.top_p < 1.0;
+    if (top == INFINITY) {
+        for (int j = 0; j < w.n; ++j) zs[j * 64 + lane] = settle(zs[j * 64 + lane], true);
+        lds_order();
+        top = 0.f;
+    }
     w.top = top;
-    w.inv = cut_k || cut_p ? bins_per_unit(top, -group_max<64>(-bottom), x.T, 64.f) : 0.f;
+    w.inv = 0.f;
+    if (cut_k || cut_p) {
+        float bottom = INFINITY;
+        for (int j = 0; j < w.n; ++j) {
+            const float z = zs[j * 64 + lane];
+            bottom = z == -INFINITY ? bottom : fminf(bottom, z);
+        }
+        w.inv = bins_per_unit(top, -group_max<64>(-bottom), x.T, 64.f);
+    }
     u64 edge = 0;
     if (cut_k) {
         auto in = [](float z, int) { return z > -INFINITY; };                    // (-inf: no mass, behind every other class)
         auto one = [](float) { return (u64)1; };
         const u64 bins = bins_of(w, s, in, one);
         const u64 run = scan<64>(bins), past = __ballot((int)run >= x.top_k);
-        const int at = past ? (int)__builtin_ctzll(past) : 63, n = (int)from_lane(run, at);
+        const int at = past ? (int)__builtin_ctzll(past) : 63, n = (int)at_lane(run, at);
         if (n <= 64) {
             // few enough for a class a lane: everything else is done there
             int count = 0;
@@ -438,7 +506,7 @@ template <int DT> __device__ __forceinline__ void choose_wave(const Choice& g, c
             lds_order();
             const u64 mine = s.place[lane];
             if (lane < n) zl = __uint_as_float((unsigned)(mine >> 32));
-            choose_lanes<64>(g, x, zl, lane < n ? key_of(zl) : 0u, (int)(unsigned)mine, top, false, true);
+            choose_lanes<64>(g, x, zl, lane < n ? key_of(zl) : 0u, (int)(unsigned)mine, top, false, true, &chosen);
             return;
         }
         edge = find_edge(w, bins, (double)x.top_k, s, in, one);
@@ -449,7 +517,7 @@ template <int DT> __device__ __forceinline__ void choose_wave(const Choice& g, c
         auto in = [&](float z, int j) { return z > -INFINITY && stays(z, j); };
         auto weight = [&](float z) { return units(mass_of(z, top, x.c), scale); };
         const u64 bins = bins_of(w, s, in, weight);
-        const u64 to = find_edge(w, bins, x.top_p * (double)from_lane(scan<64>(bins), 63), s, in, weight);
+        const u64 to = find_edge(w, bins, x.top_p * (double)at_lane(scan<64>(bins), 63), s, in, weight);
         edge = max(edge, to);
     }
     auto mass = [&](int j) {
@@ -457,38 +525,23 @@ template <int DT> __device__ __forceinline__ void choose_wave(const Choice& g, c
         const double a = mass_of(z, top, x.c);
         return stays(z, j) && a >= x.min_p ? a : 0.0;
     };
-    // where the running mass passes the goal: in which quarter of the slots, then of that quarter's, down to one slot
-    double before = 0.0, goal = 0.0, total = 0.0;
-    int from = 0, to = w.n;
-    for (bool first = true;; first = false) {
-        const int q = (to - from + 3) >> 2;
-        double v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            v[r] = 0.0;
-            for (int j = from + r * q; j < min(to, from + (r + 1) * q); ++j) v[r] += mass(j);
-        }
-        sums4(v);
-        if (first) {
-            total = v[0] + v[1] + v[2] + v[3];
-            goal = fmin(x.u * total, total * (1.0 - 0x1p-50));
-        }
-        int pick = 0;
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-            if (pick == k && before + v[k] <= goal && from + (k + 1) * q < to) { before += v[k]; ++pick; }
-        from += pick * q;
-        to = min(to, from + q);
-        if (q == 1) break;
+    // The kept mass of every slot: slot r * q + i goes to lane 16 r + i, so that lanes are in slot order
+    const int q = (w.n + 3) >> 2;
+    double slot = 0.0;
+    for (int i = 0; i < q; ++i) {
+        const double v0 = mass(i), v1 = q + i < w.n ? mass(q + i) : 0.0, v2 = 2 * q + i < w.n ? mass(2 * q + i) : 0.0,
+                     v3 = 3 * q + i < w.n ? mass(3 * q + i) : 0.0;
+        const double sums = row_sums(v0, v1, v2, v3);
+        if ((lane & 15) == i) slot = sums;
     }
-    const double mine = mass(from), run = before + scan<64>(mine);
+    const double slots = scan<64>(slot), total = at_lane(slots, 63), goal = x.u * total;
+    const u64 with = __ballot(slot > 0.0), over = __ballot(slot > 0.0 && slots > goal);
+    const int at = over ? (int)__builtin_ctzll(over) : 63 - (int)__builtin_clzll(with);
+    const int j = (at >> 4) * q + (at & 15);
+    const double mine = mass(j), run = at_lane(slots - slot, at) + scan<64>(mine);
     const u64 can = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && run > goal);
-    int hit = past ? (int)__builtin_ctzll(past) : can ? 63 - (int)__builtin_clzll(can) : -1;
-    for (int j = w.n; hit < 0 && --j >= 0;) {   // rounding led to a slot without mass: the last class that has some
-        const u64 who = __ballot(mass(j) > 0.0);
-        if (who) { hit = 63 - (int)__builtin_clzll(who); from = j; }
-    }
-    if (lane == hit) give(g, x.b, x.f, from * 64 + lane, (float)(log2_mass(zs[from * 64 + lane], top, x.c) * LN2 - log_from1(total)));
+    const int hit = past ? (int)__builtin_ctzll(past) : 63 - (int)__builtin_clzll(can);
+    chosen.add(g, x, j * 64 + hit, at_lane(log2_mass(zs[j * 64 + lane], top, x.c), hit), total);
 }
 
 // --------------------------------------------------------------------------------------- any block, any number of classes
@@ -574,7 +627,7 @@ template <int TH, class Each> __device__ __forceinline__ u64 team_edge(double go
 // The draw among classes i0 .. i1 of a block, as weights in index order: the first at which `before` + the running weight
 // passes `goal` (u == 0: the first with any mass, also one that is under half a unit).  `total`: the kept mass in units.
 template <int TH, int DT>
-__device__ __forceinline__ void team_draw(const Choice& g, const Block& x, float top, u64 edge, double scale, int i0, int i1, u64 before,
+__device__ __forceinline__ void team_draw(const Choice& g, const Block& x, float top, bool inf, u64 edge, double scale, int i0, int i1, u64 before,
                                           u64 goal, u64 total, TeamLds& s) {
     const int t = TH == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
     const int per = (i1 - i0 + TH - 1) / TH, from = min(i1, i0 + t * per), to = min(i1, from + per);
@@ -585,18 +638,19 @@ __device__ __forceinline__ void team_draw(const Choice& g, const Block& x, float
     };
     u64 own = 0, all;
     bool any;
-    for (int i = from; i < to; ++i) own += weight(i, load1<DT>(g.z, x.at + i), any);
+    auto z_at = [&](int i) { return settle(load1<DT>(g.z, x.at + i), inf); };
+    for (int i = from; i < to; ++i) own += weight(i, z_at(i), any);
     if (x.u == 0.0) { before = 0; goal = 0; }
     u64 run = before + team_scan<TH>(own, s, all) - own;
     if (own && run <= goal && run + own > goal) {
         int hit = from;
         for (int i = from; i < to; ++i) {
-            const u64 w = weight(i, load1<DT>(g.z, x.at + i), any);
+            const u64 w = weight(i, z_at(i), any);
             run += w;
             if (w) hit = i;
             if (w && run > goal) break;
         }
-        const double y = log2_mass(load1<DT>(g.z, x.at + hit), top, x.c);
+        const double y = log2_mass(z_at(hit), top, x.c);
         give(g, x.b, x.f, hit, (float)(y * LN2 - log_from1((double)total / scale)));
     }
 }
@@ -624,25 +678,28 @@ template <int TH, int DT> __device__ void choose_team(const Choice& g, const Blo
         if (t == 0) give(g, x.b, x.f, -1, no_number());
         return;
     }
+    const bool inf = top == INFINITY;
+    if (inf) top = 0.f;
+    auto z_at = [&](int i) { return settle(load1<DT>(g.z, x.at + i), inf); };
     const double scale = unit_scale(x.K);
     u64 edge = 0;
     if (x.top_k > 0 && x.top_k < x.K)
         edge = team_edge<TH>((double)x.top_k, 0, s, [&](auto f) {
             for (int i = t; i < x.K; i += TH) {
-                const float z = load1<DT>(g.z, x.at + i);
+                const float z = z_at(i);
                 if (z > -INFINITY) f(place_of(key_of(z), (unsigned)i), 1);
             }
         });
     u64 sum = 0, total;
     for (int i = t; i < x.K; i += TH) {
-        const float z = load1<DT>(g.z, x.at + i);
+        const float z = z_at(i);
         if (place_of(key_of(z), (unsigned)i) >= edge) sum += units(mass_of(z, top, x.c), scale);
     }
     team_scan<TH>(sum, s, total);
     if (x.top_p < 1.0) {
         const u64 to = team_edge<TH>(x.top_p * (double)total, 0, s, [&](auto f) {
             for (int i = t; i < x.K; i += TH) {
-                const float z = load1<DT>(g.z, x.at + i);
+                const float z = z_at(i);
                 const u64 place = place_of(key_of(z), (unsigned)i);
                 if (place >= edge) f(place, units(mass_of(z, top, x.c), scale));
             }
@@ -652,13 +709,13 @@ template <int TH, int DT> __device__ void choose_team(const Choice& g, const Blo
     if (x.top_p < 1.0 || x.min_p > 0.0) {
         sum = 0;
         for (int i = t; i < x.K; i += TH) {
-            const float z = load1<DT>(g.z, x.at + i);
+            const float z = z_at(i);
             const double a = place_of(key_of(z), (unsigned)i) >= edge ? mass_of(z, top, x.c) : 0.0;
             if (a >= x.min_p) sum += units(a, scale);
         }
         team_scan<TH>(sum, s, total);
     }
-    team_draw<TH, DT>(g, x, top, edge, scale, 0, x.K, 0, draw_goal(x.u, total), total, s);
+    team_draw<TH, DT>(g, x, top, inf, edge, scale, 0, x.K, 0, draw_goal(x.u, total), total, s);
 }
 
 // ----------------------------------------------------------------------------------- rows of features, block by block
@@ -688,15 +745,17 @@ __device__ __forceinline__ void choose_narrow(const Choice& g, const int* perm, 
         const float z = l < K ? load1<DT>(g.z, x.at + l) : -INFINITY;
         const u64 group = ((G == 64 ? 0ull : 1ull << (G & 63)) - 1) << (lane & ~(G - 1));
         const bool nan = (__ballot(z != z) & group) != 0;
-        choose_lanes<G>(g, x, z, l < K ? key_of(z) : 0u, l, group_max<G>(z), nan, live);
+        choose_lanes<G>(g, x, z, l < K ? key_of(z) : 0u, l, group_max<G>(z), nan, live, nullptr);
         if (++w == per_row) { w = 0; ++b; }
     }
 }
 
-template <int DT, int NV> __global__ void __launch_bounds__(WAVES * 64) choose_kernel(Choice g) {
-    __shared__ int s_off[MAX_LDS_FEATURES + 1], s_perm[MAX_LDS_FEATURES], s_start[5];
+template <int DT, int NV> __global__ void __launch_bounds__(WAVES * 64, 5) choose_kernel(Choice g) {
+    extern __shared__ int s_tables[];                         // of up to MAX_LDS_FEATURES features: offsets, order
+    __shared__ int s_start[5];
     __shared__ WaveMemory<NV> s_mem[WAVES];
     const bool order = g.m <= MAX_LDS_FEATURES;
+    int *s_off = s_tables, *s_perm = s_tables + g.m + 1;
     if (order) {
         for (int i = threadIdx.x; i <= g.m; i += WAVES * 64)
             s_off[i] = g.offsets ? max(0, min(g.offsets[i], g.sumK)) : i ? g.sumK : 0;
@@ -716,23 +775,25 @@ template <int DT, int NV> __global__ void __launch_bounds__(WAVES * 64) choose_k
     const unsigned i0 = (unsigned)((u64)items * wave / waves), i1 = (unsigned)((u64)items * (wave + 1) / waves);
     unsigned b = i0 / n, w = i0 - b * n;
     const int lane = threadIdx.x & 63;
+    Chosen chosen = {};
     for (unsigned it = i0; it < i1; ++it) {
         const int f = __builtin_amdgcn_readfirstlane(order ? s_perm[first + w] : (int)w);
         const int k0 = __builtin_amdgcn_readfirstlane(order ? s_off[f] : first_of(g, f));
         const int K = __builtin_amdgcn_readfirstlane(order ? max(0, s_off[f + 1] - k0) : classes_of(g, f));
-        if (!g.wide_from || K <= g.wide_from) {
-            const Block x = block_of(g, (int)b, f, k0, K);
+        if (!g.wide || K <= g.wide_from) {
+            const Block x = block_of(g, (int)__builtin_amdgcn_readfirstlane((int)b), f, k0, K);
             if (K <= 64) {
                 const float z = lane < K ? load1<DT>(g.z, x.at + lane) : -INFINITY;
-                choose_lanes<64>(g, x, z, lane < K ? key_of(z) : 0u, lane, group_max<64>(z), __any(z != z), true);
+                choose_lanes<64>(g, x, z, lane < K ? key_of(z) : 0u, lane, group_max<64>(z), __any(z != z), true, &chosen);
             } else if (K <= NV * 64) {
-                choose_wave<DT>(g, x, mem.wave.z, mem.wave.lds);
+                choose_wave<DT>(g, x, mem.wave.z, mem.wave.lds, chosen);
             } else {
                 choose_team<64, DT>(g, x, mem.team);
             }
         }
         if (++w == n) { w = 0; ++b; }
     }
+    chosen.flush(g);
 }
 
 // ------------------------------------------------------------------------------------------- very many classes, in chunks
@@ -770,7 +831,7 @@ __device__ __forceinline__ WideWs wide_ws(const Wide& w, long long block) {
 }
 // The n-th wide feature, or -1.  Every thread of the workgroup calls it.
 __device__ __forceinline__ int wide_feature(const Choice& g, int n, int* s_n) {
-    if (g.m == 1) return n == 0 && g.sumK > g.wide_from && classes_of(g, 0) > g.wide_from ? 0 : -1;
+    if (g.m == 1) return n == 0 && classes_of(g, 0) > g.wide_from ? 0 : -1;
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
         int found = -1;
@@ -792,8 +853,8 @@ struct WideBlock {
     Block x;
     WideWs s;
     int chunks;                               // of this block
-    float top, bottom;
-    bool none;
+    float top;
+    bool none, inf;
     double scale;
     float inv;
 };
@@ -826,8 +887,8 @@ __device__ __forceinline__ bool wide_block(const Choice& g, const Wide& w, long 
         top = fmaxf(top, __uint_as_float((unsigned)(t.part[i] >> 32)));
         bottom = fminf(bottom, __uint_as_float((unsigned)t.part[i]));
     }
-    o.top = top;
-    o.bottom = bottom;
+    o.inf = top == INFINITY;
+    o.top = o.inf ? 0.f : top;
     o.none = nan || o.x.bad || top == -INFINITY;
     o.inv = bins_per_unit(top, bottom, o.x.T, (float)WIDE_BINS);
     return true;
@@ -884,7 +945,7 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_bins_kernel(Choice 
     const bool mass = o.x.top_p < 1.0, count = o.x.top_k > 0;
 #pragma unroll 4
     for (int i = c * w.chunk + t; i < to; i += WT) {
-        const float z = load1<DT>(g.z, o.x.at + i);
+        const float z = settle(load1<DT>(g.z, o.x.at + i), o.inf);
         if (z > -INFINITY) {
             const int bin = wide_bin(o, z);
             if (mass) atomicAdd(&s_t.weight[bin], units(mass_of(z, o.top, o.x.c), o.scale));
@@ -956,7 +1017,7 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choi
     u64 sum = 0, any = 0;
 #pragma unroll 4
     for (int i = c * w.chunk + t; i < to; i += WT) {
-        const float z = load1<DT>(g.z, o.x.at + i);
+        const float z = settle(load1<DT>(g.z, o.x.at + i), o.inf);
         if (!(z > -INFINITY)) continue;
         const int bin = wide_bin(o, z);
         if (bin == cut.k_bin || (bin >= cut.p_from && bin <= cut.p_to)) {
@@ -1072,7 +1133,7 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_finish_kernel(Choic
         s_before = run;
     }
     __syncthreads();
-    team_draw<WT, DT>(g, o.x, o.top, edge, o.scale, s_chunk * w.chunk, min(o.x.K, (s_chunk + 1) * w.chunk), s_before, goal, total, s_t);
+    team_draw<WT, DT>(g, o.x, o.top, o.inf, edge, o.scale, s_chunk * w.chunk, min(o.x.K, (s_chunk + 1) * w.chunk), s_before, goal, total, s_t);
 }
 
 int wide_chunk(int K) {
@@ -1091,13 +1152,14 @@ bool filters_p(const clava_choice* c) { return c->top_p_t || c->top_p < 1.0; }
 
 template <int DT> int launch_choice(Choice& g, Wide& w, int max_k, hipStream_t st) {
     const unsigned blocks = (unsigned)g.B * (unsigned)g.m;
-    if (!(g.wide_from && g.m == 1 && !g.offsets)) {           // else: one feature, and it is wide
-        const unsigned grid = (blocks + WAVES - 1) / WAVES < 256 * 6 ? (blocks + WAVES - 1) / WAVES : 256 * 6;
-        if (max_k <= 1024) choose_kernel<DT, 16><<<grid, WAVES * 64, 0, st>>>(g);
-        else choose_kernel<DT, 32><<<grid, WAVES * 64, 0, st>>>(g);
+    if (g.wide_from >= 0) {
+        const unsigned grid = (blocks + WAVES - 1) / WAVES < 256 * 5 ? (blocks + WAVES - 1) / WAVES : 256 * 5;
+        const int lds = g.m <= MAX_LDS_FEATURES ? (2 * g.m + 1) * 4 : 0;
+        if (max_k <= 1024) choose_kernel<DT, 16><<<grid, WAVES * 64, lds, st>>>(g);
+        else choose_kernel<DT, 32><<<grid, WAVES * 64, lds, st>>>(g);
         CLAVA_CHECK_LAUNCH("sample_categories");
     }
-    if (g.wide_from) {
+    if (g.wide) {
         const int rows = wide_rows(w.per_row);
         for (long long row = 0; row < g.B; row += rows) {
             Choice h = g;                                     // the rows of this launch
@@ -1155,10 +1217,12 @@ int clava_sample_categories(const void* logits, int dtype, long long ld, int B, 
     const hipStream_t st = (hipStream_t)stream;
     Choice g;
     g.z = logits; g.ld = ld; g.B = B; g.m = m; g.sumK = sumK; g.offsets = offsets; g.p = *choice;
-    g.c = LOG2E / choice->temperature;
+    g.same = params_of(choice->temperature, choice->top_p, choice->min_p, choice->top_k);
+    g.tensors = choice->temperature_t || choice->top_p_t || choice->min_p_t || choice->top_k_t;
     g.u = uniforms; g.ld_u = ld_u; g.seed = seed; g.row_offset = row_offset; g.step = step_index;
     g.idx = idx; g.log_prob = log_prob;
-    g.wide_from = need ? NARROW_MAX : 0;
+    g.wide = need != 0;
+    g.wide_from = m == 1 && g.wide ? -1 : NARROW_MAX;         // (one feature: wide kernels for it, whatever its classes)
     Wide w{};
     if (need) {
         w.ws = (char*)workspace;
