@@ -48,7 +48,6 @@ struct Choice {
     const int* offsets;
     clava_choice p;
     Params same;                              // for all blocks, unless one of them is a tensor
-    bool tensors;
     const float* u; long long ld_u;
     unsigned long long seed, row_offset;
     unsigned step;
@@ -103,10 +102,13 @@ struct Block : Params {
     size_t at;
     double u;
 };
-__device__ __forceinline__ Block block_of(const Choice& g, int b, int f, int k0, int K) {
+// What a kernel is compiled for: numbers without top-k and top-p, numbers, tensors.  (Each leaves out the code and the
+// arguments that it does not need; with all of them in one, 140 scalar registers were moved to lanes and back.)
+enum { PLAIN = 0, FILTERED = 1, TENSORS = 2 };
+template <int MODE> __device__ __forceinline__ Block block_of(const Choice& g, int b, int f, int k0, int K) {
     Block x;
     static_cast<Params&>(x) = g.same;
-    if (g.tensors) {
+    if (MODE == TENSORS) {
         const clava_choice& p = g.p;
         const double T = p.temperature_t ? (double)p.temperature_t[b * p.temperature_rs + f * p.temperature_fs] : p.temperature;
         const double top_p = p.top_p_t ? (double)p.top_p_t[b * p.top_p_rs + f * p.top_p_fs] : p.top_p;
@@ -249,7 +251,7 @@ struct Chosen {
 
 // The whole choice among the classes that a group's lanes hold, one each, in index order: `z` (-inf and key 0 where a lane holds
 // none), their index, the block's maximum.  `nan`: the block holds a NaN.  All lanes of the wave come here together.
-template <int G> __device__ __forceinline__ void choose_lanes(const Choice& g, const Block& x, float z, unsigned key, int index, float top,
+template <int G, int MODE> __device__ __forceinline__ void choose_lanes(const Choice& g, const Block& x, float z, unsigned key, int index, float top,
                                                               bool nan, bool live, Chosen* chosen) {
     const int lane = threadIdx.x & 63, base = lane & ~(G - 1), l = lane & (G - 1);
     const u64 group = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1)) << base;
@@ -257,7 +259,7 @@ template <int G> __device__ __forceinline__ void choose_lanes(const Choice& g, c
     const bool inf = top == INFINITY;
     const double y = log2_mass(settle(z, inf), inf ? 0.f : top, x.c), a = exp2_nonpos(y);
     bool keep = a >= x.min_p;
-    if (__any(x.top_k > 0 || x.top_p < 1.0)) {
+    if (MODE != PLAIN && __any(x.top_k > 0 || x.top_p < 1.0)) {
         const u64 place = (u64)key << 32 | (unsigned)(63 - lane);
         const u64 sorted = sort_falling<G>(place);
         const bool in = x.top_k == 0 || l < x.top_k;
@@ -438,9 +440,9 @@ __device__ __forceinline__ double row_sums(double v0, double v1, double v2, doub
 // A block of up to 64 * (floats of zs / 64) classes.  Its logits stay in LDS: the passes over them are loops of a run-time
 // length then, and the compiler keeps no register per slot (with the block in registers the unrolled passes took 232 of them
 // and two wavefronts a SIMD).
-template <int DT> __device__ __forceinline__ void choose_wave(const Choice& g, const Block& x, float* zs, WaveLds& s, Chosen& chosen) {
+template <int DT, int MODE> __device__ __forceinline__ void choose_wave(const Choice& g, const Block& x, float* zs, WaveLds& s, Chosen& chosen) {
     const int lane = threadIdx.x & 63;
-    const bool cut_k = x.top_k > 0 && x.top_k < x.K, cut_p = x.top_p < 1.0;
+    const bool cut_k = MODE != PLAIN && x.top_k > 0 && x.top_k < x.K, cut_p = MODE != PLAIN && x.top_p < 1.0;
     WaveBlock w;
     w.z = zs;
     w.n = (x.K + 63) >> 6;
@@ -506,12 +508,12 @@ template <int DT> __device__ __forceinline__ void choose_wave(const Choice& g, c
             lds_order();
             const u64 mine = s.place[lane];
             if (lane < n) zl = __uint_as_float((unsigned)(mine >> 32));
-            choose_lanes<64>(g, x, zl, lane < n ? key_of(zl) : 0u, (int)(unsigned)mine, top, false, true, &chosen);
+            choose_lanes<64, MODE>(g, x, zl, lane < n ? key_of(zl) : 0u, (int)(unsigned)mine, top, false, true, &chosen);
             return;
         }
         edge = find_edge(w, bins, (double)x.top_k, s, in, one);
     }
-    auto stays = [&](float z, int j) { return edge == 0 || place_of(key_of(z), (unsigned)(j * 64 + lane)) >= edge; };
+    auto stays = [&](float z, int j) { return MODE == PLAIN || edge == 0 || place_of(key_of(z), (unsigned)(j * 64 + lane)) >= edge; };
     if (cut_p) {
         const double scale = unit_scale(2048);
         auto in = [&](float z, int j) { return z > -INFINITY && stays(z, j); };
@@ -729,7 +731,7 @@ template <int NV> union WaveMemory {
 };
 
 // Blocks of at most G classes, 64 / G of one row at a time; a wavefront takes a run of neighbouring items
-template <int DT, int G>
+template <int DT, int G, int MODE>
 __device__ __forceinline__ void choose_narrow(const Choice& g, const int* perm, const int* off, int n, unsigned wave, unsigned waves) {
     if (n == 0) return;
     constexpr unsigned PER = 64 / G;
@@ -741,16 +743,16 @@ __device__ __forceinline__ void choose_narrow(const Choice& g, const int* perm, 
         const int slot = (int)(w * PER) + lane / G;
         const bool live = slot < n;
         const int f = perm[live ? slot : n - 1], k0 = off[f], K = max(0, off[f + 1] - k0);
-        const Block x = block_of(g, (int)b, f, k0, K);
+        const Block x = block_of<MODE>(g, (int)b, f, k0, K);
         const float z = l < K ? load1<DT>(g.z, x.at + l) : -INFINITY;
         const u64 group = ((G == 64 ? 0ull : 1ull << (G & 63)) - 1) << (lane & ~(G - 1));
         const bool nan = (__ballot(z != z) & group) != 0;
-        choose_lanes<G>(g, x, z, l < K ? key_of(z) : 0u, l, group_max<G>(z), nan, live, nullptr);
+        choose_lanes<G, MODE>(g, x, z, l < K ? key_of(z) : 0u, l, group_max<G>(z), nan, live, nullptr);
         if (++w == per_row) { w = 0; ++b; }
     }
 }
 
-template <int DT, int NV> __global__ void __launch_bounds__(WAVES * 64, 5) choose_kernel(Choice g) {
+template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64, NV == 16 ? 5 : 4) choose_kernel(Choice g) {
     extern __shared__ int s_tables[];                         // of up to MAX_LDS_FEATURES features: offsets, order
     __shared__ int s_start[5];
     __shared__ WaveMemory<NV> s_mem[WAVES];
@@ -765,9 +767,9 @@ template <int DT, int NV> __global__ void __launch_bounds__(WAVES * 64, 5) choos
     const unsigned wave = blockIdx.x * WAVES + (threadIdx.x >> 6), waves = gridDim.x * WAVES;
     WaveMemory<NV>& mem = s_mem[threadIdx.x >> 6];
     if (order) {
-        choose_narrow<DT, 8>(g, s_perm, s_off, s_start[1], wave, waves);
-        choose_narrow<DT, 16>(g, s_perm + s_start[1], s_off, s_start[2] - s_start[1], wave, waves);
-        choose_narrow<DT, 32>(g, s_perm + s_start[2], s_off, s_start[3] - s_start[2], wave, waves);
+        choose_narrow<DT, 8, MODE>(g, s_perm, s_off, s_start[1], wave, waves);
+        choose_narrow<DT, 16, MODE>(g, s_perm + s_start[1], s_off, s_start[2] - s_start[1], wave, waves);
+        choose_narrow<DT, 32, MODE>(g, s_perm + s_start[2], s_off, s_start[3] - s_start[2], wave, waves);
     }
     const unsigned first = order ? (unsigned)s_start[3] : 0u, n = (unsigned)g.m - first;
     if (n == 0) return;
@@ -781,12 +783,12 @@ template <int DT, int NV> __global__ void __launch_bounds__(WAVES * 64, 5) choos
         const int k0 = __builtin_amdgcn_readfirstlane(order ? s_off[f] : first_of(g, f));
         const int K = __builtin_amdgcn_readfirstlane(order ? max(0, s_off[f + 1] - k0) : classes_of(g, f));
         if (!g.wide || K <= g.wide_from) {
-            const Block x = block_of(g, (int)__builtin_amdgcn_readfirstlane((int)b), f, k0, K);
+            const Block x = block_of<MODE>(g, (int)__builtin_amdgcn_readfirstlane((int)b), f, k0, K);
             if (K <= 64) {
                 const float z = lane < K ? load1<DT>(g.z, x.at + lane) : -INFINITY;
-                choose_lanes<64>(g, x, z, lane < K ? key_of(z) : 0u, lane, group_max<64>(z), __any(z != z), true, &chosen);
+                choose_lanes<64, MODE>(g, x, z, lane < K ? key_of(z) : 0u, lane, group_max<64>(z), __any(z != z), true, &chosen);
             } else if (K <= NV * 64) {
-                choose_wave<DT>(g, x, mem.wave.z, mem.wave.lds, chosen);
+                choose_wave<DT, MODE>(g, x, mem.wave.z, mem.wave.lds, chosen);
             } else {
                 choose_team<64, DT>(g, x, mem.team);
             }
@@ -863,7 +865,7 @@ __device__ __forceinline__ bool wide_block(const Choice& g, const Wide& w, long 
     const int b = (int)(block / w.per_row);
     const int f = wide_feature(g, (int)(block - (long long)b * w.per_row), s_n);
     if (f < 0) return false;
-    o.x = block_of(g, b, f, first_of(g, f), classes_of(g, f));
+    o.x = block_of<TENSORS>(g, b, f, first_of(g, f), classes_of(g, f));
     o.s = wide_ws(w, block);
     o.chunks = (o.x.K + w.chunk - 1) / w.chunk;
     o.scale = unit_scale(o.x.K);
@@ -1150,13 +1152,15 @@ int wide_rows(int per_row) { return per_row < 1024 ? 1024 / per_row : 1; }
 bool filters_k(const clava_choice* c) { return c->top_k_t || c->top_k > 0 || c->temperature_t || c->temperature < 1e-290; }
 bool filters_p(const clava_choice* c) { return c->top_p_t || c->top_p < 1.0; }
 
-template <int DT> int launch_choice(Choice& g, Wide& w, int max_k, hipStream_t st) {
+template <int DT> int launch_choice(Choice& g, Wide& w, int max_k, int mode, hipStream_t st) {
     const unsigned blocks = (unsigned)g.B * (unsigned)g.m;
     if (g.wide_from >= 0) {
         const unsigned grid = (blocks + WAVES - 1) / WAVES < 256 * 5 ? (blocks + WAVES - 1) / WAVES : 256 * 5;
         const int lds = g.m <= MAX_LDS_FEATURES ? (2 * g.m + 1) * 4 : 0;
-        if (max_k <= 1024) choose_kernel<DT, 16><<<grid, WAVES * 64, lds, st>>>(g);
-        else choose_kernel<DT, 32><<<grid, WAVES * 64, lds, st>>>(g);
+        auto* const kernel = mode == PLAIN ? (max_k <= 1024 ? choose_kernel<DT, 16, PLAIN> : choose_kernel<DT, 32, PLAIN>)
+                             : mode == FILTERED ? (max_k <= 1024 ? choose_kernel<DT, 16, FILTERED> : choose_kernel<DT, 32, FILTERED>)
+                                                : (max_k <= 1024 ? choose_kernel<DT, 16, TENSORS> : choose_kernel<DT, 32, TENSORS>);
+        kernel<<<grid, WAVES * 64, lds, st>>>(g);
         CLAVA_CHECK_LAUNCH("sample_categories");
     }
     if (g.wide) {
@@ -1218,7 +1222,8 @@ int clava_sample_categories(const void* logits, int dtype, long long ld, int B, 
     Choice g;
     g.z = logits; g.ld = ld; g.B = B; g.m = m; g.sumK = sumK; g.offsets = offsets; g.p = *choice;
     g.same = params_of(choice->temperature, choice->top_p, choice->min_p, choice->top_k);
-    g.tensors = choice->temperature_t || choice->top_p_t || choice->min_p_t || choice->top_k_t;
+    const bool tensors = choice->temperature_t || choice->top_p_t || choice->min_p_t || choice->top_k_t;
+    const int mode = tensors ? TENSORS : g.same.top_k > 0 || g.same.top_p < 1.0 ? FILTERED : PLAIN;
     g.u = uniforms; g.ld_u = ld_u; g.seed = seed; g.row_offset = row_offset; g.step = step_index;
     g.idx = idx; g.log_prob = log_prob;
     g.wide = need != 0;
@@ -1234,8 +1239,8 @@ int clava_sample_categories(const void* logits, int dtype, long long ld, int B, 
         w.p = filters_p(choice);
     }
     ProfScope prof(PROF_CHOICE, 0, (double)B * sumK * (dtype == CLAVA_DT_F32 ? 4 : 2) + 12.0 * B * m, st);
-    return dtype == CLAVA_DT_F32 ? launch_choice<CLAVA_DT_F32>(g, w, max_k, st)
-           : dtype == CLAVA_DT_BF16 ? launch_choice<CLAVA_DT_BF16>(g, w, max_k, st) : launch_choice<CLAVA_DT_F16>(g, w, max_k, st);
+    return dtype == CLAVA_DT_F32 ? launch_choice<CLAVA_DT_F32>(g, w, max_k, mode, st)
+           : dtype == CLAVA_DT_BF16 ? launch_choice<CLAVA_DT_BF16>(g, w, max_k, mode, st) : launch_choice<CLAVA_DT_F16>(g, w, max_k, mode, st);
 }
 
 }  // extern "C"
