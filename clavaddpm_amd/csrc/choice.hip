@@ -168,6 +168,9 @@ __device__ __forceinline__ int lane_here() {
     asm volatile("" : "+v"(l));
     return l;
 }
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ unsigned dpp_d(unsigned b) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
+}
 // Inclusive sums in lane order within groups of G lanes
 template <int G, class T> __device__ __forceinline__ T scan(T v) {
     if (G == 8) {
@@ -209,19 +212,23 @@ __device__ __forceinline__ int from_xor(int v, int d) {
     if (d == 8) return dpp_i<DPP_HALF_MIRROR>(dpp_i<DPP_ROW_MIRROR>(v));         // l ^ 15 ^ 7
     const auto o = d == 16 ? __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false)
                            : __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
-    return (int)(lane_here() & d ? o[0] : o[1]);
+    return (int)(__builtin_amdgcn_inverse_ballot_w64(d == 16 ? 0xffff0000ffff0000ull : 0xffffffff00000000ull) ? o[0] : o[1]);
 }
 __device__ __forceinline__ u64 from_xor(u64 v, int d) { return (u64)(unsigned)from_xor((int)(v >> 32), d) << 32 | (unsigned)from_xor((int)v, d); }
-// Bitonic sort within groups of G lanes, largest first
+// Bitonic sort within groups of G lanes, largest first.  Which lanes keep the larger one in a step is a constant, as a mask.
+constexpr u64 sort_mask(int G, int k, int d) {
+    u64 m = 0;
+    for (int l = 0; l < 64; ++l)
+        if (((l & d) == 0) == ((l & k & (G - 1)) == 0 || k == G)) m |= 1ull << l;
+    return m;
+}
 template <int G> __device__ __forceinline__ u64 sort_falling(u64 v) {
-    const int l = lane_here() & (G - 1);
 #pragma unroll
     for (int k = 2; k <= G; k *= 2)
 #pragma unroll
         for (int d = k / 2; d > 0; d /= 2) {
             const u64 o = from_xor(v, d);
-            const bool larger = ((l & d) == 0) == ((l & k) == 0 || k == G);
-            v = (v > o) == larger ? v : o;
+            v = __builtin_amdgcn_inverse_ballot_w64(~(__ballot(v > o) ^ sort_mask(G, k, d))) ? v : o;
         }
     return v;
 }
@@ -449,20 +456,24 @@ template <int DT, int MODE> __device__ __forceinline__ void choose_wave(const Ch
     float top = -INFINITY;
     unsigned largest = 0;                                    // magnitude, as bits: above infinity's for a NaN
     lds_order();
+    float bottom = INFINITY;                                 // above -inf
     auto take = [&](int j, float z) {
         largest = max(largest, __float_as_uint(z) & 0x7fffffffu);
         top = fmaxf(top, z);
+        if (MODE != PLAIN) bottom = z == -INFINITY ? bottom : fminf(bottom, z);
         zs[j * 64 + lane] = z;
     };
 #pragma unroll 4
     for (int j = 0; j < x.K >> 6; ++j) take(j, load1<DT>(g.z, x.at + j * 64 + lane));
     if (x.K & 63) {
-        const int i = (x.K & ~63) + lane;
-        float z = -INFINITY;
-        if (i < x.K) z = load1<DT>(g.z, x.at + i);
+        float z = 0.f;
+        const bool is = (x.K & ~63) + lane < x.K;
+        if (is) z = load1<DT>(g.z, x.at + (x.K & ~63) + lane);
+        largest = max(largest, __float_as_uint(z) & 0x7fffffffu);
+        z = is ? z : -INFINITY;
         top = fmaxf(top, z);
-        if (i < x.K) largest = max(largest, __float_as_uint(z) & 0x7fffffffu);
-        zs[i] = z;
+        if (MODE != PLAIN) bottom = z == -INFINITY ? bottom : fminf(bottom, z);
+        zs[(x.K & ~63) + lane] = z;
     }
     lds_order();
     top = group_max<64>(top);
@@ -473,33 +484,37 @@ template <int DT, int MODE> __device__ __forceinline__ void choose_wave(const Ch
     if (top == INFINITY) {
         for (int j = 0; j < w.n; ++j) zs[j * 64 + lane] = settle(zs[j * 64 + lane], true);
         lds_order();
-        top = 0.f;
+        top = bottom = 0.f;
     }
     w.top = top;
-    w.inv = 0.f;
-    if (cut_k || cut_p) {
-        float bottom = INFINITY;
-        for (int j = 0; j < w.n; ++j) {
-            const float z = zs[j * 64 + lane];
-            bottom = z == -INFINITY ? bottom : fminf(bottom, z);
-        }
-        w.inv = bins_per_unit(top, -group_max<64>(-bottom), x.T, 64.f);
-    }
+    w.inv = cut_k || cut_p ? bins_per_unit(top, -group_max<64>(-bottom), x.T, 64.f) : 0.f;
     u64 edge = 0;
     if (cut_k) {
         auto in = [](float z, int) { return z > -INFINITY; };                    // (-inf: no mass, behind every other class)
         auto one = [](float) { return (u64)1; };
-        const u64 bins = bins_of(w, s, in, one);
-        const u64 run = scan<64>(bins), past = __ballot((int)run >= x.top_k);
-        const int at = past ? (int)__builtin_ctzll(past) : 63, n = (int)at_lane(run, at);
+        unsigned* const count = reinterpret_cast<unsigned*>(s.bin);
+        count[lane] = 0;
+        lds_order();
+#pragma unroll 2
+        for (int j = 0; j < w.n; ++j) {
+            const float z = zs[j * 64 + lane];
+            if (z > -INFINITY) atomicAdd(&count[linear_bin(z, top, w.inv, 64)], 1u);
+        }
+        lds_order();
+        const unsigned bin = count[lane], run = scan<64>(bin);
+        const u64 past = __ballot((int)run >= x.top_k);
+        const int at = past ? (int)__builtin_ctzll(past) : 63, n = at_lane((int)run, at);
         if (n <= 64) {
             // few enough for a class a lane: everything else is done there
             int count = 0;
             float zl = -INFINITY;
+            // (its bin is at most `at`: all but -inf for the last one, whose product is inf or no number)
+            const float limit = at == 63 ? INFINITY : (float)(at + 1);
             lds_order();
+#pragma unroll 2
             for (int j = 0; j < w.n; ++j) {
                 const float z = zs[j * 64 + lane];
-                const bool is = z > -INFINITY && linear_bin(z, top, w.inv, 64) <= at;
+                const bool is = (top - z) * w.inv < limit;
                 const u64 who = __ballot(is);
                 const int pos = count + (int)__popcll(who & ((1ull << lane) - 1));
                 if (is) s.place[pos] = (u64)__float_as_uint(z) << 32 | (unsigned)(j * 64 + lane);
@@ -511,7 +526,7 @@ template <int DT, int MODE> __device__ __forceinline__ void choose_wave(const Ch
             choose_lanes<64, MODE>(g, x, zl, lane < n ? key_of(zl) : 0u, (int)(unsigned)mine, top, false, true, &chosen);
             return;
         }
-        edge = find_edge(w, bins, (double)x.top_k, s, in, one);
+        edge = find_edge(w, (u64)bin, (double)x.top_k, s, in, one);
     }
     auto stays = [&](float z, int j) { return MODE == PLAIN || edge == 0 || place_of(key_of(z), (unsigned)(j * 64 + lane)) >= edge; };
     if (cut_p) {
@@ -525,7 +540,7 @@ template <int DT, int MODE> __device__ __forceinline__ void choose_wave(const Ch
     auto mass = [&](int j) {
         const float z = zs[j * 64 + lane];
         const double a = mass_of(z, top, x.c);
-        return stays(z, j) && a >= x.min_p ? a : 0.0;
+        return (MODE != PLAIN || x.min_p > 0.0) && !(stays(z, j) && a >= x.min_p) ? 0.0 : a;
     };
     // The kept mass of every slot: slot r * q + i goes to lane 16 r + i, so that lanes are in slot order
     const int q = (w.n + 3) >> 2;
