@@ -656,16 +656,17 @@ __device__ __forceinline__ void team_draw(const Choice& g, const Block& x, float
     u64 own = 0, all;
     bool any;
     auto z_at = [&](int i) { return settle(load1<DT>(g.z, x.at + i), inf); };
+#pragma unroll 4
     for (int i = from; i < to; ++i) own += weight(i, z_at(i), any);
     if (x.u == 0.0) { before = 0; goal = 0; }
     u64 run = before + team_scan<TH>(own, s, all) - own;
     if (own && run <= goal && run + own > goal) {
         int hit = from;
+#pragma unroll 4
         for (int i = from; i < to; ++i) {
             const u64 w = weight(i, z_at(i), any);
+            if (w && run <= goal) hit = i;
             run += w;
-            if (w) hit = i;
-            if (w && run > goal) break;
         }
         const double y = log2_mass(z_at(hit), top, x.c);
         give(g, x.b, x.f, hit, (float)(y * LN2 - log_from1((double)total / scale)));
@@ -816,7 +817,7 @@ template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64
 // ------------------------------------------------------------------------------------------- very many classes, in chunks
 // Four launches over chunks of a block (top -> bins -> collect) and over blocks (finish).  Weights are integers, so that the
 // sums over chunks have no order.  Between the launches, for every wide block and in `ws`:
-constexpr int WT = 256, WIDE_BINS = 256, WIDE_LIST = 8192, WIDE_CHUNK = 4096, WIDE_CHUNKS = 1024;
+constexpr int WT = 256, WIDE_BINS = 256, WIDE_LIST = 4096, WIDE_CHUNKS = 1024;
 struct Wide {
     char* ws;
     int chunk, chunks;                        // classes of a chunk, chunks of the widest block
@@ -825,25 +826,25 @@ struct Wide {
     bool k, p;                                // some block may have top-k / top-p
 };
 struct WideWs {
-    float* range;                             // [chunks][2] largest and smallest logit above -inf (NaN: the chunk holds one)
-    unsigned* count;                          // [chunks][WIDE_BINS] classes
-    u64* mass;                                // [chunks][WIDE_BINS] and their mass
-    u64* sum;                                 // [chunks] mass that is kept whatever the edge's bin yields
-    unsigned* any;                            // [chunks] classes with such mass
     unsigned* listed;                         // places in the list
+    u64* mass;                                // [WIDE_BINS]
+    unsigned* count;                          // [WIDE_BINS] classes
     u64* list;                                // [WIDE_LIST] places in the edges' bins
+    u64* sum;                                 // [chunks] mass that is kept whatever the edge's bin yields
+    float* range;                             // [chunks][2] largest and smallest logit above -inf (NaN: the chunk holds one)
+    unsigned* any;                            // [chunks] classes with such mass
 };
-long long wide_bytes(int chunks) { return 16 + 24LL * chunks + (long long)chunks * WIDE_BINS * 12 + 8LL * WIDE_LIST; }
+long long wide_bytes(int chunks) { return 16 + 12LL * WIDE_BINS + 8LL * WIDE_LIST + 24LL * chunks; }
 __device__ __forceinline__ WideWs wide_ws(const Wide& w, long long block) {
     char* p = w.ws + block * w.stride;
     WideWs s;
     s.listed = (unsigned*)p; p += 16;
+    s.mass = (u64*)p; p += 8LL * WIDE_BINS;
+    s.count = (unsigned*)p; p += 4LL * WIDE_BINS;
+    s.list = (u64*)p; p += 8LL * WIDE_LIST;
     s.sum = (u64*)p; p += 8LL * w.chunks;
     s.range = (float*)p; p += 8LL * w.chunks;
-    s.any = (unsigned*)p; p += 8LL * w.chunks;
-    s.mass = (u64*)p; p += (long long)w.chunks * WIDE_BINS * 8;
-    s.list = (u64*)p; p += 8LL * WIDE_LIST;
-    s.count = (unsigned*)p;
+    s.any = (unsigned*)p;
     return s;
 }
 // The n-th wide feature, or -1.  Every thread of the workgroup calls it.
@@ -920,7 +921,11 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_top_kernel(Choice g
     WideBlock o;
     if (!wide_block(g, w, blockIdx.y, false, o, &s_n, s_t)) return;
     const int c = blockIdx.x, t = threadIdx.x;
-    if (c == 0 && t == 0 && (w.k || w.p)) *o.s.listed = 0;
+    if (c == 0 && (w.k || w.p)) {
+        if (t == 0) *o.s.listed = 0;
+        o.s.mass[t] = 0;
+        o.s.count[t] = 0;
+    }
     if (c >= o.chunks) return;
     float top = -INFINITY, bottom = INFINITY;
     bool nan = false;
@@ -970,8 +975,8 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_bins_kernel(Choice 
         }
     }
     __syncthreads();
-    o.s.mass[c * WIDE_BINS + t] = s_t.weight[t];
-    o.s.count[c * WIDE_BINS + t] = s_t.count[t];
+    if (s_t.weight[t]) atomicAdd(&o.s.mass[t], s_t.weight[t]);
+    if (s_t.count[t]) atomicAdd(&o.s.count[t], s_t.count[t]);
 }
 
 // Which bins the edges fall into.  Top-k's is exact; the mass that top-k leaves is known up to its bin, so top-p's goal is one
@@ -986,11 +991,8 @@ struct Cut {
 __device__ __forceinline__ Cut wide_cut(const Wide& w, const WideBlock& o, u64* s_mass, Cut* s_cut, TeamLds& s) {
     const int t = threadIdx.x;
     const bool k = o.x.top_k > 0 && o.x.top_k < o.x.K, p = o.x.top_p < 1.0;
-    u64 count = 0, mass = 0, total_count, total;
-    if (k)
-        for (int c = 0; c < o.chunks; ++c) count += o.s.count[c * WIDE_BINS + t];
-    if (p)
-        for (int c = 0; c < o.chunks; ++c) mass += o.s.mass[c * WIDE_BINS + t];
+    const u64 count = k ? o.s.count[t] : 0, mass = p ? o.s.mass[t] : 0;
+    u64 total_count, total;
     const u64 crun = team_scan<WT>(count, s, total_count), mrun = team_scan<WT>(mass, s, total);
     s_mass[t] = mrun;
     if (t == 0) *s_cut = Cut{WIDE_BINS, 0, total, total, 0, -1, WIDE_BINS};
@@ -1064,12 +1066,82 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choi
         if (s_base + i < WIDE_LIST) o.s.list[s_base + i] = s_list[i];
 }
 
+// The place of the first of the listed classes with in(place), in order, at which `before` + the running weight reaches `goal`;
+// 0 if none does.  The list's range of places is cut into 256 until at most 64 are left in one.
+template <class In, class Weight>
+__device__ __forceinline__ u64 list_edge(const u64* list, int n, double goal, u64 before, TeamLds& s, In in, Weight weight) {
+    const int t = threadIdx.x, lane = t & 63;
+    u64 lo = 0, hi = ~0ull;
+    for (;;) {
+        u64 first = ~0ull, last = 0, own = 0, count;
+        for (int i = t; i < n; i += WT) {
+            const u64 p = list[i];
+            if (p < lo || p > hi || !in(p)) continue;
+            first = min(first, p);
+            last = max(last, p);
+            ++own;
+        }
+        const u64 at = team_scan<WT>(own, s, count) - own;
+        if (count == 0) return 0;
+        if (count <= 64) {
+            // one wavefront puts them in order
+            int pos = (int)at;
+            for (int i = t; i < n; i += WT) {
+                const u64 p = list[i];
+                if (p >= lo && p <= hi && in(p)) s.weight[pos++] = p;
+            }
+            __syncthreads();
+            if (t < 64) {
+                const u64 p = sort_falling<64>(lane < (int)count ? s.weight[lane] : 0), sum = scan<64>(lane < (int)count ? weight(p) : (u64)0);
+                const u64 there = __ballot(lane < (int)count && (double)(before + sum) >= goal);
+                const u64 edge = at_lane(p, there ? (int)__builtin_ctzll(there) : (int)count - 1);
+                if (lane == 0) s.out[2] = edge;
+            }
+            __syncthreads();
+            return s.out[2];
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) {
+            first = min(first, from_xor(first, o));
+            last = max(last, from_xor(last, o));
+        }
+        __syncthreads();
+        if (lane == 0) { s.part[t >> 6] = first; s.part[WT / 64 + (t >> 6)] = last; }
+        s.weight[t] = 0;
+        __syncthreads();
+        lo = s.part[0];
+        hi = s.part[WT / 64];
+#pragma unroll
+        for (int w = 1; w < WT / 64; ++w) { lo = min(lo, s.part[w]); hi = max(hi, s.part[WT / 64 + w]); }
+        const int shift = max(0, 56 - (int)__builtin_clzll(hi - lo));           // (places differ: hi > lo)
+        for (int i = t; i < n; i += WT) {
+            const u64 p = list[i];
+            if (p >= lo && p <= hi && in(p)) atomicAdd(&s.weight[(hi - p) >> shift], weight(p));
+        }
+        __syncthreads();
+        const u64 bin = s.weight[t];
+        u64 all;
+        const u64 run = before + team_scan<WT>(bin, s, all);
+        if (t == 0) s.out[0] = 256;
+        __syncthreads();
+        if ((double)run >= goal && (t == 0 || (double)(run - bin) < goal)) { s.out[0] = (u64)t; s.out[1] = run - bin; }
+        __syncthreads();
+        if (s.out[0] == 256) return 0;
+        before = s.out[1];
+        const u64 top = hi - (s.out[0] << shift);
+        lo = max(lo, top - ((1ull << shift) - 1));
+        hi = top;
+        __syncthreads();
+    }
+}
+
 template <int DT> __global__ void __launch_bounds__(WT) wide_finish_kernel(Choice g, Wide w) {
     __shared__ int s_n;
     __shared__ TeamLds s_t;
     __shared__ u64 s_mass[WIDE_BINS];
     __shared__ Cut s_cut;
     __shared__ u64 s_sum[WIDE_CHUNKS];
+    __shared__ u64 s_list[WIDE_LIST];
     __shared__ int s_chunk;
     __shared__ u64 s_before;
     WideBlock o;
@@ -1080,52 +1152,50 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_finish_kernel(Choic
         return;
     }
     const Cut cut = wide_cut(w, o, s_mass, &s_cut, s_t);
-    const unsigned n = w.k || w.p ? *o.s.listed : 0;
-    if (n > WIDE_LIST) {                                      // too many classes in the edges' bins
+    const unsigned listed = w.k || w.p ? *o.s.listed : 0;
+    if (listed > WIDE_LIST) {                                 // too many classes in the edges' bins
         choose_team<WT, DT>(g, o.x, s_t);
         return;
     }
+    const int n = (int)listed;
+    for (int i = t; i < n; i += WT) s_list[i] = o.s.list[i];
+    __syncthreads();
     auto z_of = [&](u64 place) {
         const unsigned key = (unsigned)(place >> 32);
         return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
     };
+    auto weight = [&](u64 place) { return units(mass_of(z_of(place), o.top, o.x.c), o.scale); };
     u64 edge = 0;
     u64 k_mass = cut.m_before;
     if (cut.k_bin < WIDE_BINS) {
-        edge = team_edge<WT>((double)o.x.top_k, cut.k_before, s_t, [&](auto f) {
-            for (unsigned i = t; i < n; i += WT)
-                if (wide_bin(o, z_of(o.s.list[i])) == cut.k_bin) f(o.s.list[i], 1);
-        });
+        edge = list_edge(s_list, n, (double)o.x.top_k, cut.k_before, s_t, [&](u64 p) { return wide_bin(o, z_of(p)) == cut.k_bin; },
+                         [](u64) { return (u64)1; });
         if (cut.p_from <= cut.p_to) {
             u64 own = 0, sum;
-            for (unsigned i = t; i < n; i += WT) {
-                const float z = z_of(o.s.list[i]);
-                if (wide_bin(o, z) == cut.k_bin && o.s.list[i] >= edge) own += units(mass_of(z, o.top, o.x.c), o.scale);
-            }
+            for (int i = t; i < n; i += WT)
+                if (wide_bin(o, z_of(s_list[i])) == cut.k_bin && s_list[i] >= edge) own += weight(s_list[i]);
             team_scan<WT>(own, s_t, sum);
             k_mass += sum;
         }
     }
     if (cut.p_from <= cut.p_to) {
-        const double goal = o.x.top_p * (double)k_mass;
-        const u64 before = cut.p_from ? s_mass[cut.p_from - 1] : 0;
-        const u64 to = team_edge<WT>(goal, before, s_t, [&](auto f) {
-            for (unsigned i = t; i < n; i += WT) {
-                const u64 place = o.s.list[i];
-                const int bin = wide_bin(o, z_of(place));
-                if (bin >= cut.p_from && bin <= cut.p_to && place >= edge) f(place, units(mass_of(z_of(place), o.top, o.x.c), o.scale));
-            }
-        });
+        const u64 least = edge;
+        const u64 to = list_edge(s_list, n, o.x.top_p * (double)k_mass, cut.p_from ? s_mass[cut.p_from - 1] : 0, s_t, [&](u64 p) {
+            const int bin = wide_bin(o, z_of(p));
+            return bin >= cut.p_from && bin <= cut.p_to && p >= least;
+        }, weight);
         edge = max(edge, to);
     }
     // the kept mass of every chunk
-    __syncthreads();
-    for (int c = t; c < o.chunks; c += WT) s_sum[c] = o.x.u == 0.0 ? (u64)o.s.any[c] : o.s.sum[c];
-    __syncthreads();
     u64 mass = 0;
-    for (int c = t; c < o.chunks; c += WT) mass += o.s.sum[c];
-    for (unsigned i = t; i < n; i += WT) {
-        const u64 place = o.s.list[i];
+    for (int c = t; c < o.chunks; c += WT) {
+        const u64 m = o.s.sum[c];
+        s_sum[c] = o.x.u == 0.0 ? (u64)o.s.any[c] : m;
+        mass += m;
+    }
+    __syncthreads();
+    for (int i = t; i < n; i += WT) {
+        const u64 place = s_list[i];
         if (place < edge) continue;
         const double a = mass_of(z_of(place), o.top, o.x.c);
         if (a >= o.x.min_p && a > 0.0) {
@@ -1153,9 +1223,10 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_finish_kernel(Choic
     team_draw<WT, DT>(g, o.x, o.top, o.inf, edge, o.scale, s_chunk * w.chunk, min(o.x.K, (s_chunk + 1) * w.chunk), s_before, goal, total, s_t);
 }
 
-int wide_chunk(int K) {
-    const int c = (K + WIDE_CHUNKS - 1) / WIDE_CHUNKS;
-    return c > WIDE_CHUNK ? c : WIDE_CHUNK;
+// Classes of a chunk: 4096, or 1024 where that leaves the chip without work; more where there would be too many chunks
+int wide_chunk(int B, int K) {
+    const int c = (K + WIDE_CHUNKS - 1) / WIDE_CHUNKS, usual = (long long)B * ((K + 4095) / 4096) < 512 ? 1024 : 4096;
+    return c > usual ? c : usual;
 }
 constexpr int NARROW_MAX = 2048;              // classes that a wavefront keeps in LDS
 int wide_per_row(int m, int sumK) {
@@ -1210,7 +1281,7 @@ extern "C" {
 
 long long clava_choice_workspace_bytes(int B, int m, int sumK, int max_k) {
     if (B <= 0 || m <= 0 || sumK <= NARROW_MAX || max_k <= NARROW_MAX) return 0;
-    const int chunk = wide_chunk(sumK), chunks = (sumK + chunk - 1) / chunk;
+    const int chunk = wide_chunk(B, sumK), chunks = (sumK + chunk - 1) / chunk;
     const int per_row = wide_per_row(m, sumK), rows = wide_rows(per_row);
     return (long long)(B < rows ? B : rows) * per_row * ((wide_bytes(chunks) + 15) / 16 * 16);
 }
@@ -1246,7 +1317,7 @@ int clava_sample_categories(const void* logits, int dtype, long long ld, int B, 
     Wide w{};
     if (need) {
         w.ws = (char*)workspace;
-        w.chunk = wide_chunk(sumK);
+        w.chunk = wide_chunk(B, sumK);
         w.chunks = (sumK + w.chunk - 1) / w.chunk;
         w.per_row = wide_per_row(m, sumK);
         w.stride = (wide_bytes(w.chunks) + 15) / 16 * 16;
