@@ -915,6 +915,18 @@ __device__ __forceinline__ int wide_bin(const WideBlock& o, float z) {
     return linear_bin(z, o.top, o.inv, WIDE_BINS);
 }
 
+// f(class, logit) for the classes from .. to, eight neighbouring ones a thread
+template <int DT, class F> __device__ __forceinline__ void wide_each(const Choice& g, const Block& x, int from, int to, F f) {
+    for (int i = from + (int)threadIdx.x * 8; i < to; i += WT * 8) {
+        float z[8];
+        const int n = to - i;
+        load8<DT>(g.z, x.at + i, n, z);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) f(i + j, z[j]);
+    }
+}
+
 template <int DT> __global__ void __launch_bounds__(WT) wide_top_kernel(Choice g, Wide w) {
     __shared__ int s_n;
     __shared__ TeamLds s_t;
@@ -930,13 +942,11 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_top_kernel(Choice g
     float top = -INFINITY, bottom = INFINITY;
     bool nan = false;
     const int to = min(o.x.K, (c + 1) * w.chunk);
-#pragma unroll 4
-    for (int i = c * w.chunk + t; i < to; i += WT) {
-        const float z = load1<DT>(g.z, o.x.at + i);
+    wide_each<DT>(g, o.x, c * w.chunk, to, [&](int, float z) {
         nan |= z != z;
         top = fmaxf(top, z);
         bottom = z == -INFINITY ? bottom : fminf(bottom, z);
-    }
+    });
     top = group_max<64>(top);
     bottom = -group_max<64>(-bottom);
     if (__any(nan)) top = no_number();
@@ -965,15 +975,14 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_bins_kernel(Choice 
     __syncthreads();
     const int to = min(o.x.K, (c + 1) * w.chunk);
     const bool mass = o.x.top_p < 1.0, count = o.x.top_k > 0;
-#pragma unroll 4
-    for (int i = c * w.chunk + t; i < to; i += WT) {
-        const float z = settle(load1<DT>(g.z, o.x.at + i), o.inf);
+    wide_each<DT>(g, o.x, c * w.chunk, to, [&](int, float v) {
+        const float z = settle(v, o.inf);
         if (z > -INFINITY) {
             const int bin = wide_bin(o, z);
             if (mass) atomicAdd(&s_t.weight[bin], units(mass_of(z, o.top, o.x.c), o.scale));
             if (count) atomicAdd(&s_t.count[bin], 1u);
         }
-    }
+    });
     __syncthreads();
     if (s_t.weight[t]) atomicAdd(&o.s.mass[t], s_t.weight[t]);
     if (s_t.count[t]) atomicAdd(&o.s.count[t], s_t.count[t]);
@@ -1034,10 +1043,9 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choi
     __syncthreads();
     const int to = min(o.x.K, (c + 1) * w.chunk);
     u64 sum = 0, any = 0;
-#pragma unroll 4
-    for (int i = c * w.chunk + t; i < to; i += WT) {
-        const float z = settle(load1<DT>(g.z, o.x.at + i), o.inf);
-        if (!(z > -INFINITY)) continue;
+    wide_each<DT>(g, o.x, c * w.chunk, to, [&](int i, float v) {
+        const float z = settle(v, o.inf);
+        if (!(z > -INFINITY)) return;
         const int bin = wide_bin(o, z);
         if (bin == cut.k_bin || (bin >= cut.p_from && bin <= cut.p_to)) {
             const unsigned at = atomicAdd(&s_listed, 1u);
@@ -1051,7 +1059,7 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choi
             const double a = mass_of(z, o.top, o.x.c);
             if (a >= o.x.min_p) { sum += units(a, o.scale); any += a > 0.0; }
         }
-    }
+    });
     u64 total, n_any;
     team_scan<WT>(sum, s_t, total);
     team_scan<WT>(any, s_t, n_any);
@@ -1223,9 +1231,9 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_finish_kernel(Choic
     team_draw<WT, DT>(g, o.x, o.top, o.inf, edge, o.scale, s_chunk * w.chunk, min(o.x.K, (s_chunk + 1) * w.chunk), s_before, goal, total, s_t);
 }
 
-// Classes of a chunk: 4096, or 1024 where that leaves the chip without work; more where there would be too many chunks
+// Classes of a chunk: 4096, or 2048 where that leaves the chip without work; more where there would be too many chunks
 int wide_chunk(int B, int K) {
-    const int c = (K + WIDE_CHUNKS - 1) / WIDE_CHUNKS, usual = (long long)B * ((K + 4095) / 4096) < 512 ? 1024 : 4096;
+    const int c = (K + WIDE_CHUNKS - 1) / WIDE_CHUNKS, usual = (long long)B * ((K + 4095) / 4096) < 512 ? 2048 : 4096;
     return c > usual ? c : usual;
 }
 constexpr int NARROW_MAX = 2048;              // classes that a wavefront keeps in LDS
