@@ -10,7 +10,8 @@ namespace {
 using namespace mx4;
 
 struct Mx4Args {
-    const char* xq; const unsigned char* xs;      // [M, 64 * ks] codes, [M, 4 * ks] scales
+    const char* xq; const unsigned char* xs;      // [M, 64 * ks] codes, [M, 4 * ks] scales; or, of few rows, floats
+    int xt, K; long long ldx;                     // xt: CLAVA_DT_*
     const char* wq; const unsigned char* ws;      // [N, ...]
     const float* bias;
     int act;
@@ -74,38 +75,78 @@ template <int OUT, int C> __device__ __forceinline__ void finish(const Mx4Args& 
     }
 }
 
-// 16 rows x 32 columns a workgroup, its waves take every fourth step of K and add up through LDS.
-template <int OUT> __global__ void __launch_bounds__(256) mx4_linear_kernel(Mx4Args g, int tiles_n) {
-    __shared__ f32x4 part[3][2][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+// ---------------------------------------------------------------------------------------------------------------- few rows
+// A lane's 32 columns of a row of floats are one block: its scale and codes without another lane.
+template <int DT> __device__ __forceinline__ i32x4 pack32(const void* x, size_t at, int n, int& byte) {
+    float v[32];
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+        load8<DT>(x, at + j, n - j, v + j);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[j + k]) & 0x7fffffffu);
+    }
+    byte = scale_byte(top);
+    return i32x4{(int)pack8(v, byte), (int)pack8(v + 8, byte), (int)pack8(v + 16, byte), (int)pack8(v + 24, byte)};
+}
+
+// 16 rows x 32 columns a workgroup; its NW wavefronts take every NW-th step of K and add up through LDS.  W streams from
+// memory once, four steps of it on their way to a wavefront, and x (XT: floats or codes) comes from L2; floats are packed on
+// the way, which saves the launch that packs them and its round trip (1 x 1024 x 1024: 5.3 us in two launches).
+template <int XT, int NW, int OUT> __global__ void __launch_bounds__(NW * 64) mx4_few_kernel(Mx4Args g, int tiles_n) {
+    __shared__ f32x4 part[NW - 1][2][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
     const int m0 = (int)(blockIdx.x / (unsigned)tiles_n) * 16, n0 = (int)(blockIdx.x % (unsigned)tiles_n) * 32;
     const size_t m = min(m0 + r, g.M - 1);
     const size_t na = min(n0 + pair_row(r, 0), g.N - 1), nb = min(n0 + pair_row(r, 1), g.N - 1);
-    const char* x = g.xq + m * g.ks * 64 + q * 16;
     const char* wa = g.wq + na * g.ks * 64 + q * 16;
     const char* wb = g.wq + nb * g.ks * 64 + q * 16;
-    const unsigned char *xs = g.xs + m * g.ks * 4 + q, *was = g.ws + na * g.ks * 4 + q, *wbs = g.ws + nb * g.ks * 4 + q;
+    const unsigned char *was = g.ws + na * g.ks * 4 + q, *wbs = g.ws + nb * g.ks * 4 + q;
     f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-    for (int k = wave; k < g.ks; k += 4) {
-        const i32x4 xv = *reinterpret_cast<const i32x4*>(x + (size_t)k * 64);
-        const i32x4 av = *reinterpret_cast<const i32x4*>(wa + (size_t)k * 64), bv = *reinterpret_cast<const i32x4*>(wb + (size_t)k * 64);
-        const int sx = xs[k * 4], sa = was[k * 4], sb = wbs[k * 4];
-        const i32x8 X = {xv[0], xv[1], xv[2], xv[3], 0, 0, 0, 0}, A = {av[0], av[1], av[2], av[3], 0, 0, 0, 0},
-                    B = {bv[0], bv[1], bv[2], bv[3], 0, 0, 0, 0};
-        a = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, X, a, 4, 4, 0, sa, 0, sx);
-        b = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(B, X, b, 4, 4, 0, sb, 0, sx);
-    }
+    auto steps_from = [&](int k, auto count_t) {
+        constexpr int COUNT = decltype(count_t)::value;
+        i32x4 A[COUNT], B[COUNT], X[COUNT];
+        int sa[COUNT], sb[COUNT], sx[COUNT];
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const size_t at = (size_t)(k + i * NW);
+            A[i] = *reinterpret_cast<const i32x4*>(wa + at * 64);
+            B[i] = *reinterpret_cast<const i32x4*>(wb + at * 64);
+            sa[i] = was[at * 4];
+            sb[i] = wbs[at * 4];
+        }
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const size_t at = (size_t)(k + i * NW);
+            if (XT == CLAVA_DT_MX4) {
+                X[i] = *reinterpret_cast<const i32x4*>(g.xq + (m * g.ks + at) * 64 + q * 16);
+                sx[i] = g.xs[(m * g.ks + at) * 4 + q];
+            } else {
+                const int c = (k + i * NW) * KSTEP + q * 32;
+                X[i] = pack32<XT == CLAVA_DT_MX4 ? 0 : XT>(g.xq, m * (size_t)g.ldx + c, g.K - c, sx[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const i32x8 x = {X[i][0], X[i][1], X[i][2], X[i][3], 0, 0, 0, 0}, va = {A[i][0], A[i][1], A[i][2], A[i][3], 0, 0, 0, 0},
+                        vb = {B[i][0], B[i][1], B[i][2], B[i][3], 0, 0, 0, 0};
+            a = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, x, a, 4, 4, 0, sa[i], 0, sx[i]);
+            b = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb, x, b, 4, 4, 0, sb[i], 0, sx[i]);
+        }
+    };
+    int k = wave;
+    for (; k + 3 * NW < g.ks; k += 4 * NW) steps_from(k, std::integral_constant<int, 4>{});
+    for (; k < g.ks; k += NW) steps_from(k, std::integral_constant<int, 1>{});
     if (wave) { part[wave - 1][0][lane] = a; part[wave - 1][1][lane] = b; }
     __syncthreads();
     if (wave) return;
 #pragma unroll
-    for (int p = 0; p < 3; ++p) { a += part[p][0][lane]; b += part[p][1][lane]; }
+    for (int p = 0; p < NW - 1; ++p) { a += part[p][0][lane]; b += part[p][1][lane]; }
     float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     float bias[8];
     bias8(g, n0 + 8 * q, bias);
     finish<OUT, 8>(g, m0 + r, n0 + 8 * q, bias, v);
 }
-
 
 // ------------------------------------------------------------------------------------------------------- many rows: tiles
 __device__ __forceinline__ void dma16(const void* src, char* dst) {
@@ -250,19 +291,86 @@ __global__ void __launch_bounds__(WN * WM * 64) mx4_tile_kernel(Mx4Args g, int t
         asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WAIT) : "memory");
         multiply(smem + cur, stages - 1, std::integral_constant<int, 2>{});
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the last copies land before the LDS is someone else's
+    // the last copies land, and nobody reads the stages any more: their LDS is free
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (OUT == OUT_MX4) {
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-        const int n = n0 + (wn * TN + i) * 32 + 16 * h;
-        float bias[16];
-        bias8(g, n, bias);
-        bias8(g, n + 8, bias + 8);
+        for (int i = 0; i < TN; ++i) {
+            const int n = n0 + (wn * TN + i) * 32 + 16 * h;
+            float bias[16];
+            bias8(g, n, bias);
+            bias8(g, n + 8, bias + 8);
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+                float v[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = acc[i][j][k];
+                finish<OUT_MX4, 16>(g, m0 + (wm * TM + j) * 32 + r, n, bias, v);
+            }
+        }
+        return;
+    }
+    // A lane holds 16 columns of one row, so that stores from the accumulators touch 32 rows at a time, 16 bytes each.  Strips
+    // of 32 rows x 128 bytes (64 where a wavefront has one tile of 16-bit columns) turn in the wavefront's own LDS to whole
+    // lines (4096 x 1024 x 1024 to float32: 13.5 -> 10.6 us).
+    constexpr int SZ = OUT == CLAVA_DT_F32 ? 4 : 2, TILES = SZ == 2 && TN % 2 == 0 ? 2 : 1, ROW = 32 * TILES * SZ, PITCH = ROW + 16, PER = ROW / 16;
+    static_assert(NW * 32 * PITCH <= NS * STAGE, "the strips fit into the stages");
+    char* const strip = smem + wave * 32 * PITCH;
+#pragma unroll
+    for (int i = 0; i < TN; i += TILES) {
+        float bias[TILES][16];
+#pragma unroll
+        for (int p = 0; p < TILES; ++p) {
+            const int n = n0 + (wn * TN + i + p) * 32 + 16 * h;
+            bias8(g, n, bias[p]);
+            bias8(g, n + 8, bias[p] + 8);
+        }
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
-            float v[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = acc[i][j][k];
-            finish<OUT, 16>(g, m0 + (wm * TM + j) * 32 + r, n, bias, v);
+            for (int p = 0; p < TILES; ++p) {
+                float v[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = acc[i + p][j][k] + bias[p][k];
+                activate8(v, g.act);
+                activate8(v + 8, g.act);
+                char* const to = strip + r * PITCH + (p * 32 + 16 * h) * SZ;
+                if (SZ == 4) {
+#pragma unroll
+                    for (int k = 0; k < 16; k += 4) *reinterpret_cast<f32x4*>(to + 4 * k) = f32x4{v[k], v[k + 1], v[k + 2], v[k + 3]};
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; k += 8) {
+                        u16x8 u;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) u[e] = OUT == CLAVA_DT_BF16 ? to_bf16(v[k + e]) : to_f16(v[k + e]);
+                        *reinterpret_cast<u16x8*>(to + 2 * k) = u;
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int k = 0; k < 32 * PER / 64; ++k) {
+                const int row = k * (64 / PER) + lane / PER, c = lane % PER;
+                const int m = m0 + (wm * TM + j) * 32 + row, n = n0 + (wn * TN + i) * 32 + c * (16 / SZ);
+                const u32x4 u = *reinterpret_cast<const u32x4*>(strip + row * PITCH + c * 16);
+                if (m >= g.M || n >= g.N) continue;
+                char* const to = static_cast<char*>(g.y) + ((size_t)m * g.ldy + n) * SZ;
+                if (n + 16 / SZ <= g.N) {
+                    if (SZ == 4) *reinterpret_cast<u32x4_u4*>(to) = u;
+                    else *reinterpret_cast<u32x4_u2*>(to) = u;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16 / SZ; ++e)
+                        if (n + e < g.N) {
+                            if (SZ == 4) reinterpret_cast<unsigned*>(to)[e] = u[e];
+                            else reinterpret_cast<unsigned short*>(to)[e] = (unsigned short)(u[e / 2] >> (16 * (e & 1)));
+                        }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
     }
 }
@@ -312,17 +420,28 @@ template <int OUT> int launch_linear(const Mx4Args& g, hipStream_t st) {
         clava_set_error("linear_mx4: %d x %d outputs are more than one launch takes", g.M, g.N);
         return CLAVA_ERR_LIMIT;
     }
-    mx4_linear_kernel<OUT><<<dim3((unsigned)wgs), 256, 0, st>>>(g, tiles_n);
+    const dim3 grid((unsigned)wgs);
+    auto few = [&](auto xt) {
+        constexpr int XT = decltype(xt)::value;
+        mx4_few_kernel<XT, 8, OUT><<<grid, 512, 0, st>>>(g, tiles_n);
+    };
+    if (g.xt == CLAVA_DT_MX4) few(std::integral_constant<int, CLAVA_DT_MX4>{});
+    else if (g.xt == CLAVA_DT_F32) few(std::integral_constant<int, CLAVA_DT_F32>{});
+    else if (g.xt == CLAVA_DT_BF16) few(std::integral_constant<int, CLAVA_DT_BF16>{});
+    else few(std::integral_constant<int, CLAVA_DT_F16>{});
     return CLAVA_OK;
 }
 
+// Whether floats are packed by a launch of their own: for one tile of rows and few steps of K every workgroup packs them again
+// on the way (1 x 1024 x 1024: 4.6 us, and 5.3 in two launches; 7 x 4099 x 8001: 12.7, and 9.0)
+bool packed_first(int M, int K) { return M > 16 || K > 2048; }
 
 }  // namespace
 
 extern "C" {
 
 long long clava_linear_mx4_workspace_bytes(int M, int K, int x_dtype) {
-    return M > 0 && K > 0 && x_dtype != CLAVA_DT_MX4 ? (long long)M * steps(K) * 68 : 0;
+    return M > 0 && K > 0 && packed_first(M, K) && x_dtype != CLAVA_DT_MX4 ? (long long)M * steps(K) * 68 : 0;
 }
 
 int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_scales, const void* w_codes, const void* w_scales,
@@ -333,15 +452,18 @@ int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_sc
     CLAVA_CHECK_ARG(x_dtype >= 0 && x_dtype <= CLAVA_DT_MX4 && y_dtype >= 0 && y_dtype <= CLAVA_DT_MX4, "linear_mx4: dtypes %d, %d", x_dtype, y_dtype);
     if (M == 0) return CLAVA_OK;
     const bool x4 = x_dtype == CLAVA_DT_MX4, y4 = y_dtype == CLAVA_DT_MX4;
-    CLAVA_CHECK_ARG(x && w_codes && w_scales && y && (!y4 || y_scales) && (x4 ? x_scales : workspace), "linear_mx4: null pointer");
+    CLAVA_CHECK_ARG(x && w_codes && w_scales && y && (!y4 || y_scales) && (x4 ? x_scales != nullptr : !packed_first(M, K) || workspace), "linear_mx4: null pointer");
     CLAVA_CHECK_ARG(y4 || ldy >= N || M == 1, "linear_mx4: leading dimension %lld below %d columns", ldy, N);
-    CLAVA_CHECK_ARG((((uintptr_t)(x4 ? x : workspace) | (uintptr_t)w_codes) & 15) == 0, "linear_mx4: codes and workspace start at 16 bytes");
+    CLAVA_CHECK_ARG((((uintptr_t)(x4 ? x : packed_first(M, K) ? workspace : nullptr) | (uintptr_t)w_codes) & 15) == 0, "linear_mx4: codes and workspace start at 16 bytes");
     CLAVA_CHECK_ARG(N <= 0x7fffff00 && K <= 0x7fffff00 && M <= 0x7fffff00, "linear_mx4: M %d, N %d, K %d", M, N, K);
     const hipStream_t st = (hipStream_t)stream;
     Mx4Args g;
     g.ks = steps(K);
     g.xq = (const char*)x; g.xs = (const unsigned char*)x_scales;
-    if (!x4) {
+    g.xt = x_dtype; g.K = K; g.ldx = ldx;
+    CLAVA_CHECK_ARG(x4 || ldx >= K || M == 1, "linear_mx4: leading dimension %lld below %d columns", ldx, K);
+    if (!x4 && packed_first(M, K)) {
+        g.xt = CLAVA_DT_MX4;
         g.xq = (const char*)workspace;
         g.xs = (const unsigned char*)workspace + (size_t)M * g.ks * 64;
         const int rc = clava_mx4_pack(x, x_dtype, ldx, M, K, (void*)g.xq, (void*)g.xs, stream);

@@ -35,6 +35,10 @@ __device__ __forceinline__ unsigned pack8(const float* v, int byte) {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4_u4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 

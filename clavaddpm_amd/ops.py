@@ -466,7 +466,7 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
             y_dt, yp, ys = _dt(out, "linear_mx4: out"), out.data_ptr(), None
         if (rows, cols) != (M, N) or out.device != dev:
             _refuse(f"linear_mx4: the result is [{M},{N}] on {dev} but out is [{rows},{cols}] on {out.device}")
-    if x_dt != _MX4:
+    if x_dt != _MX4 and (M > 16 or K > 2048):
         ws = torch.empty(M * 68 * ((K + 127) // 128), device=dev, dtype=torch.uint8)      # clava_linear_mx4_workspace_bytes
     _launch(dev, "clava_linear_mx4", _function("clava_linear_mx4", "pilppppipilpiiipp"),
             xp, x_dt, ldx, xs, w.codes.data_ptr(), w.scales.data_ptr(), bp, code, yp, y_dt, ldy, ys, M, N, K,

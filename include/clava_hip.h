@@ -153,8 +153,8 @@ int clava_gemm_wgrad_f16x3_tn(const void* dy, long long pitch_dy, int shift_dy, 
  *   even, saturating at 6; a block that holds a NaN or an infinity gets scale 255 and reads as NaN.  src has row stride ld.
  * clava_mx4_unpack: dst[r * ld + c] = value(code) * 2^(scale - 127), rounded to `dtype`.
  * clava_linear_mx4: y[M,N] = act( x[M,K] . w[N,K]^T + bias[N] ), products summed in float32; w as above, x as above (x_dtype
- *   CLAVA_DT_MX4: `x` its codes, x_scales) or a float matrix of row stride ldx, which is packed into `workspace` first
- *   (clava_linear_mx4_workspace_bytes(M, K, x_dtype) bytes, 16-byte aligned).  The result as `y` (y_dtype, row stride ldy) or,
+ *   CLAVA_DT_MX4: `x` its codes, x_scales) or a float matrix of row stride ldx, which is packed as clava_mx4_pack does, into
+ *   `workspace` (clava_linear_mx4_workspace_bytes(M, K, x_dtype) bytes, 16-byte aligned; NULL where that is 0).  The result as `y` (y_dtype, row stride ldy) or,
  *   with y_dtype CLAVA_DT_MX4, packed again (`y` its codes, y_scales; for the next layer).  codes pointers are 16-byte
  *   aligned.  dtype: CLAVA_DT_*; act: CLAVA_ACT_*_. */
 int clava_mx4_pack(const void* src, int dtype, long long ld, long long rows, int cols, void* codes, void* scales, void* stream);
