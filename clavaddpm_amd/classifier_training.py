@@ -628,7 +628,7 @@ class ClassifierTrainer:
             self._snap = None
             blocks = _blocks(self.classifier)[0]
             sp.usable = bool(ClassifierSplitState.wide(blocks)) and all(b[2] == ACT_RELU or abs(b[3] - 0.01) < 1e-12 for b in blocks)
-        ok = (sp.usable and not sp.disabled and split_nets.get_gemm_mode() == "f16x3" and os.environ.get("CLAVA_CLF_SPLIT", "1") != "0"
+        ok = (sp.usable and not sp.disabled and split_nets.get_gemm_mode() != "f32" and os.environ.get("CLAVA_CLF_SPLIT", "1") != "0"
               and B % 32 == 0 and _tr.wgrad_split_ok(B, GRAD_SPLITS))
         return sp if ok else None
 

@@ -111,7 +111,7 @@ class Trainer:
     def _split_state(self):
         """The split-f16 state when that layer-kernel family is selected and the stack has hidden blocks to run on it."""
         from .. import split_nets
-        if split_nets.get_gemm_mode() != "f16x3" or len(self.diffusion._denoise_fn.mlp.blocks) < 2:
+        if split_nets.get_gemm_mode() == "f32" or len(self.diffusion._denoise_fn.mlp.blocks) < 2:
             return None
         if getattr(self, "_force_f32", 0) > 0:
             return None

@@ -11,7 +11,9 @@ The calibration batch depends only on the weights, never on the rows being sampl
 is bit-identical.  If any intermediate still leaves the float16 range the kernels raise an overflow flag and the
 caller reruns the chain on the float32 kernels (`GaussianMultinomialDiffusion._run_chain`).
 
-`set_gemm_mode("f32")` (or CLAVA_GEMM=f32) selects the float32-input MFMA kernels for the sampling loop instead.
+`set_gemm_mode("f32")` (or CLAVA_GEMM=f32) selects the float32-input MFMA kernels for the sampling loop instead,
+`set_gemm_mode("mx4")` microscaled 4-bit operands in the denoiser's hidden blocks (mx4_nets.py: a draft, not float32 accuracy;
+training runs as under "f16x3").
 """
 import ctypes
 import math
@@ -22,7 +24,7 @@ import torch
 from . import _lib, _native, ops
 from ._lib import ACT_LEAKY, ACT_NONE
 
-_MODES = ("f16x3", "f32")
+_MODES = ("f16x3", "f32", "mx4")
 _mode = os.environ.get("CLAVA_GEMM", "f16x3")
 if _mode not in _MODES:
     raise _lib.ClavaHipError(f"CLAVA_GEMM={_mode!r}: expected one of {_MODES}")
@@ -40,7 +42,8 @@ fallback_count = 0        # chains that left the float16 range and were rerun on
 
 
 def set_gemm_mode(mode):
-    """'f16x3' (default): split-f16 layers on the f16 matrix cores; 'f32': the float32-input MFMA kernels."""
+    """'f16x3' (default): split-f16 layers on the f16 matrix cores; 'f32': the float32-input MFMA kernels; 'mx4': the denoiser's
+    hidden blocks on microscaled 4-bit operands (sampling only)."""
     global _mode
     if mode not in _MODES:
         raise ValueError(f"gemm mode must be one of {_MODES}")

@@ -21,7 +21,7 @@ import ctypes
 import numpy as np
 import torch
 
-from .. import _lib, _native, split_nets
+from .. import _lib, _native, mx4_nets, ops, split_nets
 from .._lib import c_int, c_u64, check, lib, ptr, require_cuda, stream_ptr
 from . import schedule as _schedule
 from .modules import run_stack, time_embed_forward, timestep_embedding
@@ -174,9 +174,17 @@ class GaussianMultinomialDiffusion(torch.nn.Module):
               "clava_multinomial_step_f32")
         return out, lp
 
-    def p_sample_index(self, model_out_cat, idx_t, t, uniforms=None, return_log_prob=False):
-        """`p_sample` (`:468-472`) on index state: x_{t-1} indices (and optionally log p(x_{t-1} | x_t), `p_pred` `:457-466`)."""
-        return self._categorical_step(0, model_out_cat, idx_t, t, uniforms, return_log_prob)
+    def p_sample_index(self, model_out_cat, idx_t, t, uniforms=None, return_log_prob=False, *, choice=None, seed=0, row_offset=0, step_index=0):
+        """`p_sample` (`:468-472`) on index state: x_{t-1} indices (and optionally log p(x_{t-1} | x_t), `p_pred` `:457-466`).
+        With a `CategoryChoice` the classes are drawn from that posterior as it filters it, from `uniforms` [B, m] (one per
+        row and column; None: the generator keyed by (seed, row_offset + row, column, step_index))."""
+        if choice is None:
+            return self._categorical_step(0, model_out_cat, idx_t, t, uniforms, return_log_prob)
+        _, lp = self._categorical_step(0, model_out_cat, idx_t, t, None, True)
+        u = uniforms.to(lp.device).float() if uniforms is not None else None
+        idx = ops.sample_categories(lp, u, self._offsets_i32, int(self.num_classes.max()), seed=seed, row_offset=row_offset,
+                                    step_index=step_index, **choice.arguments(self._m, lp.device))
+        return idx, lp if return_log_prob else None
 
     def q_sample_index(self, idx_0, t, uniforms=None):
         """`q_sample` (`:518-523`) on index state."""
@@ -249,6 +257,8 @@ class GaussianMultinomialDiffusion(torch.nn.Module):
                 u = noise["u"][:n_steps].to(dev).float().contiguous()
                 c.uniforms = u.data_ptr()
                 keep.append(u)
+        if split_nets.get_gemm_mode() == "mx4":
+            return keep + self._run_chain_mx4(c, x, idx, ws, bs, acts, den_emb, guidance, ys, noise)
         if split_nets.get_gemm_mode() == "f16x3":
             done = self._run_chain_f16x3(c, x, idx, ws, bs, acts, den_emb, guidance, cls_emb, keep)
             if done:
@@ -263,6 +273,67 @@ class GaussianMultinomialDiffusion(torch.nn.Module):
                                            ctypes.c_longlong(int(n_ws)), stream_ptr()), "clava_sample_chain_f32")
         keep.append(wsbuf)
         return keep  # caller keeps these alive until it synchronises
+
+    def _denoiser_input(self, x, idx):
+        """[B, n_num + sum K] float32: the numeric state and the log-one-hot of the categorical one."""
+        n, sk = self.num_numerical_features, self._sum_k
+        B = x.shape[0]
+        x_in = torch.empty((B, n + sk), device=x.device, dtype=torch.float32)
+        x_in[:, :n] = x
+        if self.has_cat and B:
+            check(lib().clava_cat_onehot_image_f32(c_int(B), c_int(self._m), c_int(sk), ptr(self._offsets_i32), ptr(idx), ptr(x_in[:, n:]),
+                                                   ctypes.c_longlong(n + sk), stream_ptr()), "clava_cat_onehot_image_f32")
+        return x_in
+
+    def _gauss_step(self, sched, out, x, grad, noise, x_in, t, x_is_f32, seed, row_offset, step):
+        """Numeric columns of one reverse step with one t for all rows, in place; x_in: the next denoiser input, or None."""
+        B, n = x.shape
+        if B * n:
+            check(lib().clava_gauss_step_f32(ctypes.byref(sched), c_int(B), c_int(n), ptr(out), c_int(out.stride(0)), ptr(x), ptr(grad), c_int(n),
+                                             ptr(noise), ptr(x_in), c_int(x_in.stride(0) if x_in is not None else 0), None, None, c_int(t),
+                                             c_int(x_is_f32), c_u64(seed), c_u64(row_offset), ctypes.c_uint(step), stream_ptr()),
+                  "clava_gauss_step_f32")
+
+    def _run_chain_mx4(self, c, x, idx, ws, bs, acts, den_emb, guidance, ys, noise):
+        """The chain with the denoiser's hidden blocks on 4-bit operands: the same step kernels and noise keys, a launch at a time."""
+        dev, B, n, m, sk = x.device, x.shape[0], self.num_numerical_features, self._m, self._sum_k
+        stack = mx4_nets.Mx4Stack(ws, bs, acts)
+        buffers = stack.buffers(B)
+        x_in = self._denoiser_input(x, idx)
+        nz = noise["noise"].to(dev).double().contiguous() if noise is not None else None
+        u = noise["u"].to(dev).float().contiguous() if noise is not None and self.has_cat else None
+        seed, row_offset = int(c.seed), int(c.row_offset)
+        for s in range(int(c.n_steps)):
+            t = int(c.t_start) - s
+            step = self.num_timesteps - 1 - t
+            out = stack.forward(x_in, den_emb[t], buffers)
+            grad = guidance(x.float(), torch.full((B,), t, device=dev, dtype=torch.long), y=ys).contiguous() if guidance is not None else None
+            self._gauss_step(c.sched, out, x, grad, nz[s] if nz is not None else None, x_in if n else None, t,
+                             1 if s == 0 and c.first_step_f32 else 0, seed, row_offset, step)
+            if self.has_cat:
+                image, logits = x_in[:, n:], out[:, n:]
+                check(lib().clava_multinomial_step_f32(ctypes.byref(c.sched), c_int(0), c_int(B), c_int(m), c_int(sk), ptr(self._offsets_i32),
+                                                       ptr(self._log_k), ptr(logits), c_int(out.stride(0)), ptr(idx), ptr(idx),
+                                                       ptr(u[s]) if u is not None else None, c_int(sk), ptr(image), c_int(x_in.stride(0)), None,
+                                                       c_int(0), None, c_int(t), c_u64(seed), c_u64(row_offset), ctypes.c_uint(step),
+                                                       stream_ptr()), "clava_multinomial_step_f32")
+        return [stack, buffers, x_in, nz, u]
+
+    def _choose_last(self, x, idx, choice, noise, seed, row_offset, t_start, steps_before):
+        """The step t = 0 with its categorical columns drawn by `choice`; the numeric ones as in any chain."""
+        fn = self._denoise_fn
+        ws, bs, acts = self._denoiser_stack()
+        emb = time_embed_forward(fn.time_embed, torch.zeros(1, device=x.device, dtype=torch.long), fn.dim_t)
+        out = run_stack(ws, bs, acts, self._denoiser_input(x, idx), rowadd0=emb)[-1]
+        t = torch.zeros(x.shape[0], device=x.device, dtype=torch.long)
+        step = self.num_timesteps - 1
+        u = noise["u_choice"] if noise is not None else None
+        n = self.num_numerical_features
+        chosen, _ = self.p_sample_index(out[:, n:], idx, t, u, choice=choice, seed=seed, row_offset=row_offset, step_index=step)
+        nz = noise["noise"][steps_before].to(x.device).double().contiguous() if noise is not None else None
+        first = steps_before == 0 and t_start == step and not (noise is not None and noise["z0"].dtype == torch.float64)
+        self._gauss_step(self._c_schedule(), out, x, None, nz, None, 0, 1 if first else 0, seed, row_offset, step)
+        idx.copy_(chosen)
 
     def _run_chain_f16x3(self, c, x, idx, ws, bs, acts, den_emb, guidance, cls_emb, keep):
         """The same chain with every Linear on the f16 matrix cores (split-f16, float32-level accuracy: csrc/split.h).
@@ -366,8 +437,12 @@ class GaussianMultinomialDiffusion(torch.nn.Module):
 
     @torch.no_grad()
     def sample(self, num_samples, y_dist, model_kwargs=None, cond_fn=None, *, noise=None, seed=None, row_offset=0, n_steps=None, t_start=None,
-               idx_start=None):
-        """Unconditional chain (`:1026-1070`); returns (sample float64 CPU [b, n_num + m], {'y': labels})."""
+               idx_start=None, choice=None):
+        """Unconditional chain (`:1026-1070`); returns (sample float64 CPU [b, n_num + m], {'y': labels}).
+        `choice`: a `CategoryChoice` that the last step (t = 0) draws the categorical columns with (an injected `noise` then
+        holds its uniforms [b, m] as "u_choice")."""
+        if choice is not None and not self.has_cat:
+            raise ValueError("choice: the table has no categorical columns")
         dev = self._device()
         b = num_samples
         seed = _fresh_seed() if seed is None else seed
@@ -387,13 +462,24 @@ class GaussianMultinomialDiffusion(torch.nn.Module):
             # from y_dist above: `conditional_sampling` (pipeline_utils.py:1001-1012) passes its own `classes` there and
             # records them as the rows' clusters
             labels = self._guidance_labels(model_kwargs, b) if cond_fn is not None else out_dict['y']
-            keep = self._run_chain(x, idx, cond_fn, labels, noise, seed, row_offset, n_steps, t_start)
+            if choice is None:
+                keep = self._run_chain(x, idx, cond_fn, labels, noise, seed, row_offset, n_steps, t_start)
+            else:
+                last = self.num_timesteps - 1 if t_start is None else int(t_start)
+                if n_steps is not None and int(n_steps) != last + 1:
+                    raise ValueError(f"choice applies to the step t = 0, which {n_steps} steps from t = {last} do not end with")
+                keep = self._run_chain(x, idx, None, labels, noise, seed, row_offset, last, t_start) if last and b else []
+                if b:
+                    self._choose_last(x, idx, choice, noise, seed, row_offset, last, last)
         else:
             if self.has_cat:
                 raise NotImplementedError("a Python cond_fn with categorical columns is not supported")
             keep = self._run_chain_python_guidance(x, cond_fn, model_kwargs or {}, noise, seed, row_offset, n_steps)
         sample = self._finish(x, idx)
         del keep
+        if choice is not None:      # a column without a class to choose (its logits were not numbers): NaN, like a numeric one
+            cats = sample[:, self.num_numerical_features:]
+            cats[cats < 0] = float("nan")
         return sample, out_dict
 
     def _guidance_labels(self, model_kwargs, b):
@@ -435,7 +521,7 @@ class GaussianMultinomialDiffusion(torch.nn.Module):
                                              ctypes.c_uint(s), stream_ptr()), "clava_gauss_step_f32")
         return [nz, emb]
 
-    def sample_all(self, num_samples, batch_size, y_dist, ddim=False, model_kwargs=None, cond_fn=None, *, seed=None):
+    def sample_all(self, num_samples, batch_size, y_dist, ddim=False, model_kwargs=None, cond_fn=None, *, seed=None, choice=None):
         """Batches of `batch_size` until `num_samples` rows exist (`:1072-1099`): returns (x_gen CPU [N, n_num+m], y_gen CPU [N]);
         raises FoundNANsError if any sampled row has a NaN."""
         if ddim:
@@ -446,7 +532,7 @@ class GaussianMultinomialDiffusion(torch.nn.Module):
         num_generated = 0
         while num_generated < num_samples:
             sample, out_dict = self.sample(b, y_dist, model_kwargs=model_kwargs, cond_fn=cond_fn, seed=seed,
-                                           row_offset=num_generated)
+                                           row_offset=num_generated, choice=choice)
             mask_nan = torch.any(sample.isnan(), dim=1)
             sample = sample[~mask_nan]
             out_dict['y'] = out_dict['y'].cpu()[~mask_nan]
