@@ -655,21 +655,31 @@ __device__ __forceinline__ void team_draw(const Choice& g, const Block& x, float
     };
     u64 own = 0, all;
     bool any;
-    auto z_at = [&](int i) { return settle(load1<DT>(g.z, x.at + i), inf); };
-#pragma unroll 4
-    for (int i = from; i < to; ++i) own += weight(i, z_at(i), any);
+    // f(class, weight, logit) for the thread's run, eight loads at a time
+    auto run_over = [&](auto f) {
+        for (int i = from; i < to; i += 8) {
+            float z[8];
+            const int n = to - i;
+            load8<DT>(g.z, x.at + i, n, z);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) {
+                    const float v = settle(z[j], inf);
+                    f(i + j, weight(i + j, v, any), v);
+                }
+        }
+    };
+    run_over([&](int, u64 w, float) { own += w; });
     if (x.u == 0.0) { before = 0; goal = 0; }
     u64 run = before + team_scan<TH>(own, s, all) - own;
     if (own && run <= goal && run + own > goal) {
         int hit = from;
-#pragma unroll 4
-        for (int i = from; i < to; ++i) {
-            const u64 w = weight(i, z_at(i), any);
-            if (w && run <= goal) hit = i;
+        float z = top;
+        run_over([&](int i, u64 w, float v) {
+            if (w && run <= goal) { hit = i; z = v; }
             run += w;
-        }
-        const double y = log2_mass(z_at(hit), top, x.c);
-        give(g, x.b, x.f, hit, (float)(y * LN2 - log_from1((double)total / scale)));
+        });
+        give(g, x.b, x.f, hit, (float)(log2_mass(z, top, x.c) * LN2 - log_from1((double)total / scale)));
     }
 }
 template <int TH, int DT> __device__ void choose_team(const Choice& g, const Block& x, TeamLds& s) {
@@ -746,14 +756,26 @@ template <int NV> union WaveMemory {
     TeamLds team;
 };
 
-// Blocks of at most G classes, 64 / G of one row at a time; a wavefront takes a run of neighbouring items
+// The items of a wavefront: a run of neighbouring ones, or, where there are fewer items than wavefronts, at most one, behind
+// the `before` ones that other kinds of items have given to the first wavefronts (1 row of 50 columns: no wavefront has two)
+__device__ __forceinline__ void items_of(unsigned items, unsigned before, unsigned wave, unsigned waves, unsigned& from, unsigned& to) {
+    if (items >= waves) {
+        from = (unsigned)((u64)items * wave / waves);
+        to = (unsigned)((u64)items * (wave + 1) / waves);
+    } else {
+        from = (wave + waves - before % waves) % waves;
+        to = min(from + 1, items);
+    }
+}
+// Blocks of at most G classes, 64 / G of one row at a time; returns the number of items
 template <int DT, int G, int MODE>
-__device__ __forceinline__ void choose_narrow(const Choice& g, const int* perm, const int* off, int n, unsigned wave, unsigned waves) {
-    if (n == 0) return;
+__device__ __forceinline__ unsigned choose_narrow(const Choice& g, const int* perm, const int* off, int n, unsigned before, unsigned wave, unsigned waves) {
+    if (n == 0) return 0;
     constexpr unsigned PER = 64 / G;
     const int lane = threadIdx.x & 63, l = lane & (G - 1);
     const unsigned per_row = ((unsigned)n + PER - 1) / PER, items = per_row * (unsigned)g.B;
-    const unsigned i0 = (unsigned)((u64)items * wave / waves), i1 = (unsigned)((u64)items * (wave + 1) / waves);
+    unsigned i0, i1;
+    items_of(items, before, wave, waves, i0, i1);
     unsigned b = i0 / per_row, w = i0 - b * per_row;
     for (unsigned it = i0; it < i1; ++it) {
         const int slot = (int)(w * PER) + lane / G;
@@ -766,6 +788,7 @@ __device__ __forceinline__ void choose_narrow(const Choice& g, const int* perm, 
         choose_lanes<G, MODE>(g, x, z, l < K ? key_of(z) : 0u, l, group_max<G>(z), nan, live, nullptr);
         if (++w == per_row) { w = 0; ++b; }
     }
+    return items;
 }
 
 template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64, NV == 16 ? 5 : 4) choose_kernel(Choice g) {
@@ -782,15 +805,16 @@ template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64
     }
     const unsigned wave = blockIdx.x * WAVES + (threadIdx.x >> 6), waves = gridDim.x * WAVES;
     WaveMemory<NV>& mem = s_mem[threadIdx.x >> 6];
+    unsigned before = 0;
     if (order) {
-        choose_narrow<DT, 8, MODE>(g, s_perm, s_off, s_start[1], wave, waves);
-        choose_narrow<DT, 16, MODE>(g, s_perm + s_start[1], s_off, s_start[2] - s_start[1], wave, waves);
-        choose_narrow<DT, 32, MODE>(g, s_perm + s_start[2], s_off, s_start[3] - s_start[2], wave, waves);
+        before += choose_narrow<DT, 8, MODE>(g, s_perm, s_off, s_start[1], before, wave, waves);
+        before += choose_narrow<DT, 16, MODE>(g, s_perm + s_start[1], s_off, s_start[2] - s_start[1], before, wave, waves);
+        before += choose_narrow<DT, 32, MODE>(g, s_perm + s_start[2], s_off, s_start[3] - s_start[2], before, wave, waves);
     }
     const unsigned first = order ? (unsigned)s_start[3] : 0u, n = (unsigned)g.m - first;
     if (n == 0) return;
-    const unsigned items = n * (unsigned)g.B;
-    const unsigned i0 = (unsigned)((u64)items * wave / waves), i1 = (unsigned)((u64)items * (wave + 1) / waves);
+    unsigned i0, i1;
+    items_of(n * (unsigned)g.B, before, wave, waves, i0, i1);
     unsigned b = i0 / n, w = i0 - b * n;
     const int lane = threadIdx.x & 63;
     Chosen chosen = {};
@@ -828,13 +852,14 @@ struct Wide {
 struct WideWs {
     unsigned* listed;                         // places in the list
     u64* mass;                                // [WIDE_BINS]
+    u64* chunk_mass;                          // [chunks][WIDE_BINS]
     unsigned* count;                          // [WIDE_BINS] classes
     u64* list;                                // [WIDE_LIST] places in the edges' bins
     u64* sum;                                 // [chunks] mass that is kept whatever the edge's bin yields
     float* range;                             // [chunks][2] largest and smallest logit above -inf (NaN: the chunk holds one)
     unsigned* any;                            // [chunks] classes with such mass
 };
-long long wide_bytes(int chunks) { return 16 + 12LL * WIDE_BINS + 8LL * WIDE_LIST + 24LL * chunks; }
+long long wide_bytes(int chunks) { return 16 + 12LL * WIDE_BINS + 8LL * WIDE_LIST + 24LL * chunks + 8LL * WIDE_BINS * chunks; }
 __device__ __forceinline__ WideWs wide_ws(const Wide& w, long long block) {
     char* p = w.ws + block * w.stride;
     WideWs s;
@@ -843,6 +868,7 @@ __device__ __forceinline__ WideWs wide_ws(const Wide& w, long long block) {
     s.count = (unsigned*)p; p += 4LL * WIDE_BINS;
     s.list = (u64*)p; p += 8LL * WIDE_LIST;
     s.sum = (u64*)p; p += 8LL * w.chunks;
+    s.chunk_mass = (u64*)p; p += 8LL * WIDE_BINS * w.chunks;
     s.range = (float*)p; p += 8LL * w.chunks;
     s.any = (unsigned*)p;
     return s;
@@ -985,6 +1011,7 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_bins_kernel(Choice 
     });
     __syncthreads();
     if (s_t.weight[t]) atomicAdd(&o.s.mass[t], s_t.weight[t]);
+    if (mass) o.s.chunk_mass[c * WIDE_BINS + t] = s_t.weight[t];
     if (s_t.count[t]) atomicAdd(&o.s.count[t], s_t.count[t]);
 }
 
@@ -1027,6 +1054,10 @@ __device__ __forceinline__ Cut wide_cut(const Wide& w, const WideBlock& o, u64* 
     return c;
 }
 
+// Whether a chunk's kept mass follows from its bins: then `collect` takes no exponentials (they are most of its time: 64 x
+// 131071 23 us with them).  Not where min-p cuts inside a bin, nor for u = 0, which counts classes.
+__device__ __forceinline__ bool mass_is_binned(const Block& x) { return x.top_p < 1.0 && x.min_p == 0.0 && x.u > 0.0; }
+
 template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choice g, Wide w) {
     __shared__ int s_n;
     __shared__ TeamLds s_t;
@@ -1042,6 +1073,7 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choi
     if (t == 0) s_listed = 0;
     __syncthreads();
     const int to = min(o.x.K, (c + 1) * w.chunk);
+    const bool binned = mass_is_binned(o.x);
     u64 sum = 0, any = 0;
     wide_each<DT>(g, o.x, c * w.chunk, to, [&](int i, float v) {
         const float z = settle(v, o.inf);
@@ -1055,12 +1087,13 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choi
                 const unsigned far = atomicAdd(o.s.listed, 1u);
                 if (far < WIDE_LIST) o.s.list[far] = place;
             }
-        } else if (bin < cut.sure) {
+        } else if (bin < cut.sure && !binned) {
             const double a = mass_of(z, o.top, o.x.c);
             if (a >= o.x.min_p) { sum += units(a, o.scale); any += a > 0.0; }
         }
     });
     u64 total, n_any;
+    if (binned) sum = t < cut.sure ? o.s.chunk_mass[c * WIDE_BINS + t] : 0;
     team_scan<WT>(sum, s_t, total);
     team_scan<WT>(any, s_t, n_any);
     const unsigned n = min(s_listed, 1024u);
