@@ -24,16 +24,15 @@ __global__ void __launch_bounds__(256) mx4_pack_kernel(const void* __restrict__ 
     if ((g & 3) == 0) scales[i >> 2] = (unsigned char)byte;
 }
 
-// E2M1 codes of one lane (8 of them) times 2^(byte - 127); 255 reads as NaN
+// E2M1 codes of one lane (8 of them) times 2^(byte - 127); 255 reads as NaN.  The conversion takes the scale as a float32, which
+// 2^-127 is not as a normal number: half of twice it is.
 __device__ __forceinline__ void unpack8(unsigned q, int byte, float* v) {
+    const float s = byte == 255 ? __uint_as_float(0x7fc00000u) : byte ? __uint_as_float((unsigned)byte << 23) : 0x1p-126f, half = byte ? 1.f : 0.5f;
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1),
+               c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 3);
+    const float u[8] = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const unsigned c = (q >> (4 * j)) & 15u, m = c & 7u;
-        // 0, 1/2, then 1.m with exponent bias 1
-        const float a = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-        const float s = byte == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(a, byte - 127);
-        v[j] = c & 8u ? -s : s;
-    }
+    for (int j = 0; j < 8; ++j) v[j] = u[j] * s * half;
 }
 
 template <int DT>
