@@ -366,7 +366,7 @@ def _launch(dev, name, f, *args):
 class Mx4Tensor:
     """A [rows, cols] matrix in microscaled 4-bit form (see include/clava_hip.h): `codes` uint8 [rows, Kp / 2] and `scales`
     uint8 [rows, Kp / 32], Kp = cols rounded up to 128.  The codes behind the last column have to be zero."""
-    __slots__ = ("codes", "scales", "rows", "cols", "device")
+    __slots__ = ("rows", "cols", "device", "codes_ptr", "scales_ptr", "_codes", "_scales", "_buf")
 
     def __init__(self, codes, scales, cols):
         cols = int(cols)
@@ -383,16 +383,41 @@ class Mx4Tensor:
         self.device = codes.device
         if scales.device != self.device:
             _refuse(f"Mx4Tensor: scales are on {scales.device}, codes on {self.device}")
-        if codes.data_ptr() & 15:
+        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
+        if self.codes_ptr & 15:
             _refuse("Mx4Tensor: codes must start at a multiple of 16 bytes")
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+        self._codes, self._scales, self.rows, self.cols, self._buf = codes, scales, rows, cols, None
+
+    # (mx4_empty's two parts share one allocation; the views are made when somebody looks at them)
+    @property
+    def codes(self):
+        if self._codes is None:
+            n = self.rows * 64 * ((self.cols + 127) // 128)
+            self._codes = self._buf[:n].view(self.rows, -1) if n else self._buf.view(0, 64 * ((self.cols + 127) // 128))
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            steps = (self.cols + 127) // 128
+            n = self.rows * 64 * steps
+            self._scales = self._buf[n:].view(self.rows, -1) if n else self._buf.view(0, 4 * steps)
+        return self._scales
 
 
 def mx4_empty(rows, cols, device):
     """An uninitialised Mx4Tensor, for `out`."""
-    steps = (int(cols) + 127) // 128
-    return Mx4Tensor(torch.empty((rows, 64 * steps), device=device, dtype=torch.uint8),
-                     torch.empty((rows, 4 * steps), device=device, dtype=torch.uint8), cols)
+    q = Mx4Tensor.__new__(Mx4Tensor)
+    steps = (cols + 127) // 128
+    if cols < 1 or rows < 0:
+        _refuse(f"mx4_empty: [{rows}, {cols}]")
+    buf = torch.empty(rows * 68 * steps, device=device, dtype=torch.uint8)
+    if not buf.is_cuda:
+        require_cuda(buf)
+    q.rows, q.cols, q.device, q._buf, q._codes, q._scales = rows, cols, buf.device, buf, None, None
+    q.codes_ptr = buf.data_ptr()
+    q.scales_ptr = q.codes_ptr + rows * 64 * steps
+    return q
 
 
 def mx4_pack(x, out=None):
@@ -405,7 +430,7 @@ def mx4_pack(x, out=None):
     elif (out.rows, out.cols) != (rows, cols) or out.device != x.device:
         _refuse(f"mx4_pack: x is [{rows},{cols}] on {x.device} but out is [{out.rows},{out.cols}] on {out.device}")
     _launch(out.device, "clava_mx4_pack", _function("clava_mx4_pack", "pillippp"),
-            x.data_ptr(), dt, ld, rows, cols, out.codes.data_ptr(), out.scales.data_ptr())
+            x.data_ptr(), dt, ld, rows, cols, out.codes_ptr, out.scales_ptr)
     return out
 
 
@@ -419,7 +444,7 @@ def mx4_unpack(q, dtype=torch.float32, out=None):
     if (rows, cols) != (q.rows, q.cols) or out.device != q.device:
         _refuse(f"mx4_unpack: q is [{q.rows},{q.cols}] on {q.device} but out is [{rows},{cols}] on {out.device}")
     _launch(q.device, "clava_mx4_unpack", _function("clava_mx4_unpack", "pplipilp"),
-            q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(), _dt(out, "mx4_unpack: out"), ld)
+            q.codes_ptr, q.scales_ptr, rows, cols, out.data_ptr(), _dt(out, "mx4_unpack: out"), ld)
     return out
 
 
@@ -434,7 +459,7 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
         _refuse(f"linear_mx4: unknown activation {act!r}")
     N, dev, ws = w.rows, w.device, None
     if isinstance(x, Mx4Tensor):
-        M, K, ldx, x_dt, xp, xs = x.rows, x.cols, 0, _MX4, x.codes.data_ptr(), x.scales.data_ptr()
+        M, K, ldx, x_dt, xp, xs = x.rows, x.cols, 0, _MX4, x.codes_ptr, x.scales_ptr
     else:
         M, K, ldx = _matrix(x, "linear_mx4: x")
         x_dt, xp, xs = _dt(x, "linear_mx4: x"), x.data_ptr(), None
@@ -460,7 +485,7 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
         y_dt, ldy, yp, ys = _DT[out_dtype], N, out.data_ptr(), None
     else:
         if isinstance(out, Mx4Tensor):
-            rows, cols, ldy, y_dt, yp, ys = out.rows, out.cols, 0, _MX4, out.codes.data_ptr(), out.scales.data_ptr()
+            rows, cols, ldy, y_dt, yp, ys = out.rows, out.cols, 0, _MX4, out.codes_ptr, out.scales_ptr
         else:
             rows, cols, ldy = _matrix(out, "linear_mx4: out")
             y_dt, yp, ys = _dt(out, "linear_mx4: out"), out.data_ptr(), None
@@ -469,7 +494,7 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
     if x_dt != _MX4 and (M > 16 or K > 2048):
         ws = torch.empty(M * 68 * ((K + 127) // 128), device=dev, dtype=torch.uint8)      # clava_linear_mx4_workspace_bytes
     _launch(dev, "clava_linear_mx4", _function("clava_linear_mx4", "pilppppipilpiiipp"),
-            xp, x_dt, ldx, xs, w.codes.data_ptr(), w.scales.data_ptr(), bp, code, yp, y_dt, ldy, ys, M, N, K,
+            xp, x_dt, ldx, xs, w.codes_ptr, w.scales_ptr, bp, code, yp, y_dt, ldy, ys, M, N, K,
             None if ws is None else ws.data_ptr())
     return out
 
