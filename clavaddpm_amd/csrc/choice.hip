@@ -233,6 +233,37 @@ template <int G> __device__ __forceinline__ u64 sort_falling(u64 v) {
     return v;
 }
 
+// The same in one register: both lanes of a pair see the pair, the mask says which keeps the larger
+template <int G> __device__ __forceinline__ unsigned sort_falling(unsigned v) {
+#pragma unroll
+    for (int k = 2; k <= G; k *= 2)
+#pragma unroll
+        for (int d = k / 2; d > 0; d /= 2) {
+            unsigned o;
+            if (d >= 16) {
+                const auto pair = d == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+                v = pair[0];
+                o = pair[1];
+            } else o = (unsigned)from_xor((int)v, d);
+            v = __builtin_amdgcn_inverse_ballot_w64(sort_mask(G, k, d)) ? max(v, o) : min(v, o);
+        }
+    return v;
+}
+// The places (key, 63 - lane) of a group's lanes, largest first.  They are sorted by the leading 26 or 27 bits of max - z with
+// the lane below them, in one register; where that has left two in the wrong order (bits that agree: under one block in a
+// hundred at 50 classes) or max - z is no number, by all their bits.
+template <int G> __device__ __forceinline__ u64 sort_places(unsigned key, float z, float top) {
+    const int lane = threadIdx.x & 63, l = lane & (G - 1);
+    const u64 place = (u64)key << 32 | (unsigned)(63 - lane);
+    if (G < 32) return sort_falling<G>(place);
+    const unsigned first = sort_falling<G>((~(__float_as_uint(top - z) << 1) & ~(unsigned)(G - 1)) | (unsigned)(G - 1 - l));
+    const int from = (lane | (G - 1)) - (int)(first & (G - 1));
+    const u64 sorted = (u64)(unsigned)__shfl((int)key, from, 64) << 32 | (unsigned)(63 - from);
+    constexpr int WAVE_SHR1 = 0x138;
+    const u64 above = dpp_d<WAVE_SHR1>(sorted);
+    return __any(l > 0 && above < sorted) ? sort_falling<G>(place) : sorted;
+}
+
 // What a wavefront has chosen, a block a lane: the logarithms and the stores of 64 blocks are done together
 struct Chosen {
     unsigned n, out;
@@ -267,8 +298,7 @@ template <int G, int MODE> __device__ __forceinline__ void choose_lanes(const Ch
     const double y = log2_mass(settle(z, inf), inf ? 0.f : top, x.c), a = exp2_nonpos(y);
     bool keep = a >= x.min_p;
     if (MODE != PLAIN && __any(x.top_k > 0 || x.top_p < 1.0)) {
-        const u64 place = (u64)key << 32 | (unsigned)(63 - lane);
-        const u64 sorted = sort_falling<G>(place);
+        const u64 place = (u64)key << 32 | (unsigned)(63 - lane), sorted = sort_places<G>(key, z, top);
         const bool in = x.top_k == 0 || l < x.top_k;
         const double as = from_lane(a, 63 - (int)(unsigned)sorted);
         const double w = in ? as : 0.0, run = scan<G>(w);
@@ -447,7 +477,9 @@ __device__ __forceinline__ double row_sums(double v0, double v1, double v2, doub
 // A block of up to 64 * (floats of zs / 64) classes.  Its logits stay in LDS: the passes over them are loops of a run-time
 // length then, and the compiler keeps no register per slot (with the block in registers the unrolled passes took 232 of them
 // and two wavefronts a SIMD).
-template <int DT, int MODE> __device__ __forceinline__ void choose_wave(const Choice& g, const Block& x, float* zs, WaveLds& s, Chosen& chosen) {
+// `ahead` is called once the logits are there.
+template <int DT, int MODE, class Ahead>
+__device__ __forceinline__ void choose_wave(const Choice& g, const Block& x, float* zs, WaveLds& s, Chosen& chosen, Ahead ahead) {
     const int lane = threadIdx.x & 63;
     const bool cut_k = MODE != PLAIN && x.top_k > 0 && x.top_k < x.K, cut_p = MODE != PLAIN && x.top_p < 1.0;
     WaveBlock w;
@@ -477,6 +509,7 @@ template <int DT, int MODE> __device__ __forceinline__ void choose_wave(const Ch
     }
     lds_order();
     top = group_max<64>(top);
+    ahead();
     if (__any(largest > 0x7f800000u) || x.bad || top == -INFINITY) {
         if (lane == 0) give(g, x.b, x.f, -1, no_number());
         return;
@@ -819,21 +852,32 @@ template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64
     const int lane = threadIdx.x & 63;
     Chosen chosen = {};
     for (unsigned it = i0; it < i1; ++it) {
+        const int row = __builtin_amdgcn_readfirstlane((int)b);
         const int f = __builtin_amdgcn_readfirstlane(order ? s_perm[first + w] : (int)w);
         const int k0 = __builtin_amdgcn_readfirstlane(order ? s_off[f] : first_of(g, f));
         const int K = __builtin_amdgcn_readfirstlane(order ? max(0, s_off[f + 1] - k0) : classes_of(g, f));
+        if (++w == n) { w = 0; ++b; }
+        // A lane a 64-byte piece of the row from the next block on: its lines are on their way while this one is worked on
+        // (20000 x 50 filtered 960 -> 890 us; to the end of a block as wide as this one 920; the next logits and uniforms kept
+        // in registers 1240, from 48 of them spilled)
+        float touched = 0.f;
+        auto ahead = [&] {
+            if (!order || it + 1 == i1) return;
+            const int at = __builtin_amdgcn_readfirstlane(s_off[s_perm[first + w]]) + lane * (DT == CLAVA_DT_F32 ? 16 : 32);
+            if (at < g.sumK) touched = load1<DT>(g.z, (size_t)b * g.ld + at);
+        };
         if (!g.wide || K <= g.wide_from) {
-            const Block x = block_of<MODE>(g, (int)__builtin_amdgcn_readfirstlane((int)b), f, k0, K);
+            const Block x = block_of<MODE>(g, row, f, k0, K);
             if (K <= 64) {
                 const float z = lane < K ? load1<DT>(g.z, x.at + lane) : -INFINITY;
                 choose_lanes<64, MODE>(g, x, z, lane < K ? key_of(z) : 0u, lane, group_max<64>(z), __any(z != z), true, &chosen);
             } else if (K <= NV * 64) {
-                choose_wave<DT, MODE>(g, x, mem.wave.z, mem.wave.lds, chosen);
+                choose_wave<DT, MODE>(g, x, mem.wave.z, mem.wave.lds, chosen, ahead);
             } else {
                 choose_team<64, DT>(g, x, mem.team);
             }
         }
-        if (++w == n) { w = 0; ++b; }
+        asm volatile("" : : "v"(touched));
     }
     chosen.flush(g);
 }
