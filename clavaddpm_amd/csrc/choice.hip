@@ -27,18 +27,18 @@ struct Params {
     double c, top_p, min_p;                   // log2(e) / T; in (0, 1], 1: off; in [0, 1]
     float T;                                  // for bin widths only
     int top_k;                                // 0: off
-    bool bad;                                 // the temperature is negative or no number
+    bool bad;                                 // the temperature is negative, or one of them is no number
 };
 __host__ __device__ __forceinline__ Params params_of(double T, double top_p, double min_p, int top_k) {
     Params p;
-    p.bad = !(T >= 0.0);
+    p.bad = !(T >= 0.0) || top_p != top_p || min_p != min_p;
     if (!(T >= 1e-290)) { T = 1.0; top_k = 1; }              // 0, and what 1 / T has no float64 for
     p.c = LOG2E / T;
     if (p.c < 1e-290) p.c = 1e-290;                          // (an infinite T: -inf * c stays -inf)
     p.T = T < 1e30 ? (float)T : 1e30f;
     p.top_k = top_k > 0 ? top_k : 0;
     p.min_p = min_p > 0.0 ? (min_p < 1.0 ? min_p : 1.0) : 0.0;
-    p.top_p = top_p < 1.0 ? (top_p > 1e-290 ? top_p : 1e-290) : 1.0;       // the first of the order always stays; NaN: off
+    p.top_p = top_p < 1.0 ? (top_p > 1e-290 ? top_p : 1e-290) : 1.0;       // the first of the order always stays
     return p;
 }
 
@@ -52,8 +52,8 @@ struct Choice {
     unsigned long long seed, row_offset;
     unsigned step;
     int* idx; float* log_prob;
-    bool wide;                                // blocks with more than wide_from classes belong to the wide_* kernels
-    int wide_from;
+    bool wide;                                // blocks of more than wide_from, at most wide_to classes belong to the wide_* kernels
+    int wide_from, wide_to;
 };
 
 // 2^y for y <= 0 (NaN and what is below float64: 0): n = rint(y), 2^(y - n) by its power series in base 2, ln2^k / k!, up to
@@ -866,7 +866,7 @@ template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64
             const int at = __builtin_amdgcn_readfirstlane(s_off[s_perm[first + w]]) + lane * (DT == CLAVA_DT_F32 ? 16 : 32);
             if (at < g.sumK) touched = load1<DT>(g.z, (size_t)b * g.ld + at);
         };
-        if (!g.wide || K <= g.wide_from) {
+        if (!g.wide || K <= g.wide_from || K > g.wide_to) {
             const Block x = block_of<MODE>(g, row, f, k0, K);
             if (K <= 64) {
                 const float z = lane < K ? load1<DT>(g.z, x.at + lane) : -INFINITY;
@@ -924,7 +924,8 @@ __device__ __forceinline__ int wide_feature(const Choice& g, int n, int* s_n) {
         const int lane = threadIdx.x;
         int found = -1;
         for (int f0 = 0; f0 < g.m && found < 0; f0 += 64) {
-            u64 who = __ballot(f0 + lane < g.m && classes_of(g, min(f0 + lane, g.m - 1)) > g.wide_from);
+            const int K = classes_of(g, min(f0 + lane, g.m - 1));
+            u64 who = __ballot(f0 + lane < g.m && K > g.wide_from && K <= g.wide_to);
             const int c = (int)__popcll(who);
             if (n < c) {
                 for (int k = 0; k < n; ++k) who &= who - 1;
@@ -1318,6 +1319,8 @@ int wide_per_row(int m, int sumK) {
     const int most = sumK / (NARROW_MAX + 1);
     return most < m ? most : m;
 }
+// The widest block that the wide kernels take, and have workspace for: wider ones than the caller said are a wavefront's
+int wide_most(int m, int sumK, int max_k) { return m == 1 || max_k > sumK ? sumK : max_k; }
 // Rows of one launch: 1024 wide blocks fill the chip, and the workspace need not hold more
 int wide_rows(int per_row) { return per_row < 1024 ? 1024 / per_row : 1; }
 bool filters_k(const clava_choice* c) { return c->top_k_t || c->top_k > 0 || c->temperature_t || c->temperature < 1e-290; }
@@ -1366,7 +1369,7 @@ extern "C" {
 
 long long clava_choice_workspace_bytes(int B, int m, int sumK, int max_k) {
     if (B <= 0 || m <= 0 || sumK <= NARROW_MAX || max_k <= NARROW_MAX) return 0;
-    const int chunk = wide_chunk(B, sumK), chunks = (sumK + chunk - 1) / chunk;
+    const int most = wide_most(m, sumK, max_k), chunk = wide_chunk(B, most), chunks = (most + chunk - 1) / chunk;
     const int per_row = wide_per_row(m, sumK), rows = wide_rows(per_row);
     return (long long)(B < rows ? B : rows) * per_row * ((wide_bytes(chunks) + 15) / 16 * 16);
 }
@@ -1399,11 +1402,12 @@ int clava_sample_categories(const void* logits, int dtype, long long ld, int B, 
     g.idx = idx; g.log_prob = log_prob;
     g.wide = need != 0;
     g.wide_from = m == 1 && g.wide ? -1 : NARROW_MAX;         // (one feature: wide kernels for it, whatever its classes)
+    g.wide_to = wide_most(m, sumK, max_k);
     Wide w{};
     if (need) {
         w.ws = (char*)workspace;
-        w.chunk = wide_chunk(B, sumK);
-        w.chunks = (sumK + w.chunk - 1) / w.chunk;
+        w.chunk = wide_chunk(B, g.wide_to);
+        w.chunks = (g.wide_to + w.chunk - 1) / w.chunk;
         w.per_row = wide_per_row(m, sumK);
         w.stride = (wide_bytes(w.chunks) + 15) / 16 * 16;
         w.k = filters_k(choice);

@@ -1,5 +1,5 @@
 // Dense layer over microscaled 4-bit matrices: y[m][n] = act( sum over blocks of 2^(ex + ew) * (sum of 32 products of codes)
-// + bias[n] ).  v_mfma_scale_f32_16x16x128 takes both scales with the codes and accumulates in float32.  W is the instruction's
+// + bias[n] ).  v_mfma_scale_f32 (16x16x128, 32x32x64) takes both scales with the codes and accumulates in float32.  W is the instruction's
 // first operand, so that a lane ends up with neighbouring columns of one row of y.
 #include <type_traits>
 
@@ -432,6 +432,7 @@ template <int OUT> int launch_linear(const Mx4Args& g, hipStream_t st) {
     return CLAVA_OK;
 }
 
+constexpr int MOST_COLUMNS = 1 << 25;         // 255 rows of codes are inside the 32 bits of a lane's source then
 // Whether floats are packed by a launch of their own: for one tile of rows and few steps of K every workgroup packs them again
 // on the way (1 x 1024 x 1024: 4.6 us, and 5.3 in two launches; 7 x 4099 x 8001: 12.7, and 9.0)
 bool packed_first(int M, int K) { return M > 16 || K > 2048; }
@@ -456,6 +457,10 @@ int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_sc
     CLAVA_CHECK_ARG(y4 || ldy >= N || M == 1, "linear_mx4: leading dimension %lld below %d columns", ldy, N);
     CLAVA_CHECK_ARG((((uintptr_t)(x4 ? x : packed_first(M, K) ? workspace : nullptr) | (uintptr_t)w_codes) & 15) == 0, "linear_mx4: codes and workspace start at 16 bytes");
     CLAVA_CHECK_ARG(N <= 0x7fffff00 && K <= 0x7fffff00 && M <= 0x7fffff00, "linear_mx4: M %d, N %d, K %d", M, N, K);
+    if (K > MOST_COLUMNS) {
+        clava_set_error("linear_mx4: %d columns are more than one call takes (%d)", K, MOST_COLUMNS);
+        return CLAVA_ERR_LIMIT;
+    }
     const hipStream_t st = (hipStream_t)stream;
     Mx4Args g;
     g.ks = steps(K);

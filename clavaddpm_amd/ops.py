@@ -425,6 +425,8 @@ def mx4_pack(x, out=None):
     that holds a NaN or an infinity reads as NaN.  No gradient is defined."""
     rows, cols, ld = _matrix(x, "mx4_pack: x")
     dt = _dt(x, "mx4_pack: x")
+    if x.requires_grad and torch.is_grad_enabled():
+        _refuse("mx4_pack has no backward: call it under torch.no_grad() or detach its input")
     if out is None:
         out = mx4_empty(rows, cols, x.device)
     elif (out.rows, out.cols) != (rows, cols) or out.device != x.device:
@@ -448,10 +450,25 @@ def mx4_unpack(q, dtype=torch.float32, out=None):
     return out
 
 
+def _span(t, cols, ld):
+    """(bytes of a row, of its stride)"""
+    return (64 * ((cols + 127) // 128),) * 2 if isinstance(t, Mx4Tensor) else (cols * t.element_size(), ld * t.element_size())
+
+
+def _overlap(a, row_a, step_a, b, row_b, step_b, rows):
+    """Whether two matrices share memory; of columns of one buffer only if they share columns."""
+    if a + (rows - 1) * step_a + row_a <= b or b + (rows - 1) * step_b + row_b <= a:
+        return False
+    if rows == 1 or step_a != step_b:
+        return True
+    d = (b - a) % step_a
+    return d < row_a or d + row_b > step_a
+
+
 def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
     """act(x @ w.T + bias) over 4-bit operands (clava_linear_mx4): `w` an Mx4Tensor [N, K], `x` an Mx4Tensor [M, K] or a float
     matrix, which is packed first.  The result is a float matrix of `out_dtype`, or whatever `out` is: a float matrix or an
-    Mx4Tensor (the next layer's operand).  No gradient is defined."""
+    Mx4Tensor (the next layer's operand); it may not overlap x.  No gradient is defined."""
     if not isinstance(w, Mx4Tensor):
         _refuse("linear_mx4: w must be an Mx4Tensor")
     code = _ACT.get(act)
@@ -491,6 +508,8 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
             y_dt, yp, ys = _dt(out, "linear_mx4: out"), out.data_ptr(), None
         if (rows, cols) != (M, N) or out.device != dev:
             _refuse(f"linear_mx4: the result is [{M},{N}] on {dev} but out is [{rows},{cols}] on {out.device}")
+        if M and _overlap(xp, *_span(x, K, ldx), yp, *_span(out, N, ldy), M):
+            _refuse("linear_mx4: out overlaps x, which is read while out is written")
     if x_dt != _MX4 and (M > 16 or K > 2048):
         ws = torch.empty(M * 68 * ((K + 127) // 128), device=dev, dtype=torch.uint8)      # clava_linear_mx4_workspace_bytes
     _launch(dev, "clava_linear_mx4", _function("clava_linear_mx4", "pilppppipilpiiipp"),
@@ -506,7 +525,7 @@ class _CChoice(ctypes.Structure):
                [(n + s, c_ll) for n in ("temperature", "top_p", "min_p", "top_k") for s in ("_rs", "_fs")]
 
 
-_CHOICE_RANGE = {"temperature": (0.0, math.inf), "top_p": (0.0, math.inf), "min_p": (0.0, 1.0), "top_k": (-math.inf, math.inf)}
+_CHOICE_RANGE = {"temperature": (0.0, math.inf), "top_p": (0.0, math.inf), "min_p": (0.0, 1.0), "top_k": (-2 ** 63, 2 ** 63)}
 
 
 def _choice_args(dev, rows, features, values):
@@ -527,8 +546,8 @@ def _choice_args(dev, rows, features, values):
             setattr(c, name + "_fs", fs)
             continue
         low, high = _CHOICE_RANGE[name]
-        if not low <= v <= high:
-            _refuse(f"sample_categories: {name} {v} outside [{low}, {high}]")
+        if not low <= v <= high or name == "top_k" and v != int(v):
+            _refuse(f"sample_categories: {name} {v}, expected {'a whole number' if name == 'top_k' else f'in [{low}, {high}]'}")
         setattr(c, name, max(-1, min(int(v), 2 ** 31 - 1)) if name == "top_k" else v)
     return c
 
@@ -541,11 +560,14 @@ def sample_categories(logits, uniforms=None, offsets=None, max_classes=None, *, 
 
     Feature f owns columns offsets[f] .. offsets[f+1] (int32 device tensor [m + 1]; None: one feature of all columns).
     `uniforms`: float32 [B, m] in [0, 1) ([B] for one feature), or None for the generator keyed by (seed, row_offset + row,
-    feature, step_index).  `max_classes`: the largest number of classes of one feature, which picks the kernels (any value is
-    safe; default: all columns).  Each parameter is a number or a device tensor (float32; top_k int32) that broadcasts to
-    [B, m].  A feature with no class left to draw (none, all logits -inf, a NaN) yields -1 and NaN."""
+    feature, step_index).  `max_classes`: the largest number of classes of one feature, which picks the kernels and the workspace
+    (any value is safe, a feature of more classes is slow; default: all columns).  Each parameter is a number or a device tensor (float32; top_k int32) that broadcasts to
+    [B, m].  A feature with no class left to draw (none, all logits -inf, a NaN) or with a parameter that is no number yields -1
+    and NaN.  A captured call repeats its own draws: give it `uniforms` that the program refills."""
     B, sumk, ld = _matrix(logits, "sample_categories: logits")
     dt = _dt(logits, "sample_categories: logits")
+    if log_prob and logits.requires_grad and torch.is_grad_enabled():
+        _refuse("sample_categories: log_prob has no backward: call it under torch.no_grad() or detach the logits")
     dev = logits.device
     m, op = 1, None
     if offsets is not None:

@@ -280,3 +280,72 @@ def test_refusals():
     for f in bad:
         with pytest.raises(ClavaHipError):
             f()
+
+
+@pytest.mark.parametrize("K", [0, 1, 5, 64, 65, 2048, 2049, 4500])
+def test_one_feature_inside_a_wider_row(K):
+    z = torch.randn((3, 5000), generator=torch.Generator().manual_seed(K))
+    u = uniforms(3, 1, K)
+    off = torch.tensor([17, 17 + K], device=DEV, dtype=torch.int32)
+    for p in ({}, {"top_k": 7, "top_p": 0.9}, {"min_p": 0.2}):
+        want = expect(z[:, 17:17 + K], u, [K], **{"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0, **p})
+        same(ops.sample_categories(z.to(DEV), u.to(DEV), off, log_prob=True, **p), want, max(K, 1))
+
+
+@pytest.mark.parametrize("B, classes", [(1100, [2100]), (530, [2100, 30, 2200])])
+def test_more_wide_rows_than_one_launch_takes(B, classes):
+    z = 2 * torch.randn((B, sum(classes)), generator=torch.Generator().manual_seed(B))
+    u = uniforms(B, len(classes), B)
+    check(z, u, classes, max(classes), top_k=40, top_p=0.9)
+    # parameters and outputs of the rows behind the first launch are theirs too
+    k = torch.from_numpy(np.random.RandomState(1).randint(1, 60, (B, 1))).int()
+    idx = ops.sample_categories(z.to(DEV), u.to(DEV), offsets(classes), top_k=k.to(DEV))
+    cut = ops.sample_categories(z[-9:].to(DEV), u[-9:].to(DEV), offsets(classes), top_k=k[-9:].to(DEV))
+    assert torch.equal(idx[-9:], cut)
+
+
+def test_more_features_than_their_table_holds():
+    classes = [1 + i % 70 for i in range(1300)] + [300, 2500]
+    z = torch.randn((2, sum(classes)), generator=torch.Generator().manual_seed(3))
+    for p in ({}, {"top_k": 3, "top_p": 0.8}):
+        check(z, uniforms(2, len(classes), 4), classes, 2500, **p)
+        check(z, uniforms(2, len(classes), 4), classes, None, **p)
+
+
+def test_features_wider_than_the_caller_said():
+    classes = [2060, 9, 2500, 6000]
+    z = torch.randn((5, sum(classes)), generator=torch.Generator().manual_seed(3))
+    for hint in (2049, 2060, 2499, 2500, 5999):
+        check(z, uniforms(5, 4, 4), classes, hint, top_k=30, top_p=0.8)
+
+
+def test_parameters_that_are_no_numbers():
+    z = torch.randn(4, 50, device=DEV)
+    for name in ("temperature", "top_p", "min_p"):
+        v = torch.tensor([[0.5], [math.nan], [0.5], [math.nan]], device=DEV)
+        idx, lp = ops.sample_categories(z, None, log_prob=True, **{name: v})
+        assert (idx[1::2] == -1).all() and lp[1::2].isnan().all() and (idx[::2] >= 0).all()
+    for bad in (dict(top_k=2.5), dict(top_k=math.inf), dict(top_k=math.nan), dict(top_p=math.nan)):
+        with pytest.raises(ClavaHipError):
+            ops.sample_categories(z, None, **bad)
+    grad = z.clone().requires_grad_()
+    with pytest.raises(ClavaHipError):
+        ops.sample_categories(grad, None, log_prob=True)
+    with torch.no_grad():
+        ops.sample_categories(grad, None, log_prob=True)
+    ops.sample_categories(grad, None)
+
+
+def test_offsets_that_pass_32_bits():
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    classes = [4, 100, 900, 3000]
+    n = sum(classes)
+    z = torch.randn((3, n), generator=torch.Generator().manual_seed(3)).bfloat16()
+    far = torch.empty((1 << 32) + n, device=DEV, dtype=torch.bfloat16).as_strided((3, n), (1 << 31, 1))
+    far.copy_(z)
+    u = uniforms(3, 4, 4).to(DEV)
+    for p in ({}, {"top_k": 30, "top_p": 0.8}):
+        a = ops.sample_categories(far, u, offsets(classes), log_prob=True, **p)
+        b = ops.sample_categories(z.to(DEV), u, offsets(classes), log_prob=True, **p)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

@@ -251,3 +251,99 @@ def test_refusals():
             f()
     with torch.no_grad():
         ops.linear_mx4(x.clone().requires_grad_(), w)
+
+
+@pytest.mark.parametrize("M, N", [(2050, 2100), (5000, 6700)])            # tiles of 128 x 128, of 256 x 256
+@pytest.mark.parametrize("K", [40, 300, 512, 1030])                       # one step of 128 columns, an odd number, whole groups of four, nine
+def test_large_products(M, N, K):
+    x, w, bias, want, mag = product_case(M, K, N, K)
+    xq, wq, b = ops.mx4_pack(x.to(DEV)), ops.mx4_pack(w.to(DEV)), bias.to(DEV)
+    y = ops.linear_mx4(x.to(DEV), wq, b, act="relu")
+    ref = np.maximum(want + bias.double().numpy(), 0)
+    assert (np.abs(y.cpu().double().numpy() - ref) <= tolerance(M, K, N, mag + np.abs(bias.numpy()), ref, torch.float32)).all()
+    assert torch.equal(y, ops.linear_mx4(xq, wq, b, act="relu"))
+    assert torch.equal(y.bfloat16(), ops.linear_mx4(xq, wq, b, act="relu", out_dtype=torch.bfloat16))
+    out, again = ops.linear_mx4(xq, wq, b, act="relu", out=ops.mx4_empty(M, N, DEV)), ops.mx4_pack(y)
+    assert torch.equal(out.codes, again.codes) and torch.equal(out.scales, again.scales)
+    big = torch.full((M + 1, N + 9), 9.0, device=DEV)
+    ops.linear_mx4(xq, wq, b, act="relu", out=big[:M, 5:5 + N])
+    assert torch.equal(big[:M, 5:5 + N], y) and (big[M] == 9).all() and (big[:, :5] == 9).all() and (big[:, 5 + N:] == 9).all()
+
+
+@pytest.mark.parametrize("M", [1, 16, 17, 64, 65])
+@pytest.mark.parametrize("K", [2047, 2048, 2049])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_and_columns_at_which_the_way_changes(M, K, dtype):
+    x, w, _, want, mag = product_case(M, K, 45, M + K, dtype)
+    wq = ops.mx4_pack(w.to(DEV))
+    wide = torch.randn(M, K + 5, device=DEV).to(dtype)
+    wide[:, 3:3 + K] = x.to(DEV)
+    y = ops.linear_mx4(wide[:, 3:3 + K], wq)
+    assert (np.abs(y.cpu().double().numpy() - want) <= tolerance(M, K, 45, mag, want, torch.float32)).all()
+    assert torch.equal(y, ops.linear_mx4(ops.mx4_pack(x.to(DEV)), wq))
+
+
+def test_result_beside_its_operand_but_not_on_it():
+    x, w = torch.randn(70, 128, device=DEV), ops.mx4_pack(torch.randn(128, 128, device=DEV))
+    want = ops.linear_mx4(x, w)
+    both = torch.cat([x, torch.zeros_like(x)], 1)
+    ops.linear_mx4(both[:, :128], w, out=both[:, 128:])
+    assert torch.equal(both[:, 128:], want)
+    stack = torch.cat([x, torch.zeros_like(x)])
+    ops.linear_mx4(stack[:70], w, out=stack[70:])
+    assert torch.equal(stack[70:], want)
+    q = ops.mx4_pack(x)
+    for f in (lambda: ops.linear_mx4(x, w, out=x), lambda: ops.linear_mx4(both[:, :128], w, out=both[:, 127:255]), lambda: ops.linear_mx4(q, w, out=q),
+              lambda: ops.linear_mx4(stack[:70], w, out=stack[69:139]), lambda: ops.linear_mx4(x[:1], w, out=x[:1]),
+              lambda: ops.mx4_pack(x.clone().requires_grad_())):
+        with pytest.raises(ClavaHipError):
+            f()
+
+
+def test_offsets_that_pass_32_bits():
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    x, w = torch.randn(66, 200, device=DEV), ops.mx4_pack(torch.randn(72, 200, device=DEV))
+    step = (1 << 32) // 60 // 128 * 128                                   # rows end past 2^32 elements
+    far = torch.empty(66 * step, device=DEV, dtype=torch.bfloat16)
+    for M in (2, 66):
+        s = step if M == 66 else 60 * step
+        xs = far.as_strided((M, 200), (s, 1))
+        xs.copy_(x[:M])
+        near = x[:M].bfloat16()
+        assert torch.equal(ops.mx4_pack(xs).codes, ops.mx4_pack(near).codes)
+        want = ops.linear_mx4(near, w, out_dtype=torch.bfloat16)
+        assert torch.equal(ops.linear_mx4(xs, w, out_dtype=torch.bfloat16), want)
+        ys = far.as_strided((M, 72), (s, 1), 300)
+        assert torch.equal(ops.linear_mx4(near, w, out=ys), want)
+        ops.mx4_unpack(ops.mx4_pack(want), out=ys)
+        assert torch.equal(ys, ops.mx4_unpack(ops.mx4_pack(want), dtype=torch.bfloat16))
+    del far, xs, ys
+    # more than 2^31 groups of eight columns: several launches
+    rows = (1 << 31) // 16 + 5
+    q = ops.mx4_empty(rows, 128, DEV)
+    tail = torch.randn(9, 128, device=DEV)
+    flat = torch.zeros(rows, 128, device=DEV, dtype=torch.bfloat16)
+    flat[-9:] = tail
+    ops.mx4_pack(flat, out=q)
+    ref = ops.mx4_pack(tail.bfloat16())
+    assert torch.equal(q.codes[-9:], ref.codes) and torch.equal(q.scales[-9:], ref.scales) and (q.codes[-20:-9] == 0).all()
+    ops.mx4_unpack(q, out=flat)
+    assert torch.equal(flat[-9:], ops.mx4_unpack(ref, dtype=torch.bfloat16)) and (flat[-20:-9] == 0).all()
+
+
+def test_two_streams_at_once():
+    x, y, w = torch.randn(3000, 700, device=DEV), torch.randn(9, 3001, device=DEV), ops.mx4_pack(torch.randn(1000, 700, device=DEV))
+    v = ops.mx4_pack(torch.randn(77, 3001, device=DEV))
+    want = ops.linear_mx4(x, w), ops.linear_mx4(y, v)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(5):
+        with torch.cuda.stream(a):
+            got.append((0, ops.linear_mx4(x, w)))
+        with torch.cuda.stream(b):
+            got.append((1, ops.linear_mx4(y, v)))
+    torch.cuda.synchronize()
+    for k, t in got:
+        assert torch.equal(t, want[k])

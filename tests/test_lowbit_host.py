@@ -111,3 +111,25 @@ def test_mx4_is_a_gemm_mode():
     finally:
         split_nets.set_gemm_mode(before)
     assert _lib.declared_symbols()
+
+
+def test_matrices_that_share_memory_are_told_from_columns_of_one_buffer():
+    # (start, bytes of a row, row stride) twice, rows
+    assert ops._overlap(0, 16, 64, 8, 16, 64, 4) and ops._overlap(8, 16, 64, 0, 16, 64, 4)
+    assert not ops._overlap(0, 16, 64, 16, 48, 64, 4) and not ops._overlap(16, 48, 64, 0, 16, 64, 4)
+    assert ops._overlap(0, 16, 64, 16, 49, 64, 4) and ops._overlap(0, 16, 64, 60, 8, 64, 4)
+    assert ops._overlap(0, 16, 64, 16, 16, 32, 4)                        # strides that differ
+    assert not ops._overlap(0, 16, 64, 208, 16, 32, 4) and not ops._overlap(208, 16, 32, 0, 16, 64, 4)
+    assert ops._overlap(0, 16, 16, 15, 1, 1, 1) and not ops._overlap(0, 16, 16, 16, 1, 1, 1)
+
+
+def test_more_columns_than_a_product_takes():
+    p = ctypes.c_void_p(4096)
+    assert "33554433" in c_refuses("clava_linear_mx4", "pilppppipilpiiipp", p, 3, 0, p, p, p, None, 0, p, 0, 8, None, 4, 8, (1 << 25) + 1, None)
+
+
+def test_the_workspace_is_for_blocks_as_wide_as_the_caller_says():
+    need = ops._function("clava_choice_workspace_bytes", "iiii", ops.c_ll)
+    assert need(64, 400, 10 ** 6, 5000) < need(64, 400, 10 ** 6, 10 ** 6) // 4
+    assert need(64, 400, 10 ** 6, 10 ** 6) == need(64, 400, 10 ** 6, 2 ** 31 - 1)
+    assert need(64, 1, 10 ** 6, 5000) == need(64, 1, 10 ** 6, 10 ** 6)   # one feature: its own width
