@@ -28,12 +28,13 @@ __device__ __forceinline__ void activate8(float* v, int act) {
         for (int j = 0; j < 8; ++j) v[j] = v[j] / (1.f + expf(-v[j]));
         return;
     }
-    const bool relu = act == CLAVA_ACT_RELU;
+    if (act == CLAVA_ACT_RELU) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float low = relu ? 0.f : 0.01f * v[j];
-        v[j] = v[j] <= 0.f ? low : v[j];
+        for (int j = 0; j < 8; ++j) v[j] = v[j] <= 0.f ? 0.f : v[j];
+        return;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] <= 0.f ? 0.01f * v[j] : v[j];
 }
 
 // Row of W behind row `r` of the first (odd = 0) or second tile of a pair: a lane's accumulators of the two tiles are then
@@ -407,8 +408,9 @@ template <int OUT> int launch_linear(const Mx4Args& g, hipStream_t st) {
     const int n_cols = OUT == OUT_MX4 ? g.yks * KSTEP : g.N;
     const int tiles_n = (n_cols + 31) / 32;
     // Many rows: the largest tile that still gives every CU two rounds of work (a large tile copies least per product; us for
-    // 256 x 256 / 128 x 128 / 64 x 64 tiles: 16384 x 8192 x 8192 591 / 672 / 1056, 20000 x 1024 x 1024 28.6 / 22.8 / 38.8,
-    // 4096 x 1024 x 1024 14.3 / 7.7 / 10.1, 1024 x 1024 x 1024 13.4 / 6.2 / 4.7, 256 x 4096 x 4096 30.6 / 12.9 / 8.5).
+    // 256 x 256 / 128 x 128 / 64 x 64 tiles, codes to bfloat16: 16384 x 8192 x 8192 540 / 690 / 1083, 20000 x 1024 x 1024
+    // 27.7 / 23.3 / 38.8, 4096 x 1024 x 1024 13.9 / 7.7 / 10.3, 1024 x 1024 x 1024 13.0 / 6.4 / 4.7, 256 x 4096 x 4096
+    // 30.2 / 13.0 / 8.4).
     auto tiles = [&](int t) { return (long long)((g.M + t - 1) / t) * ((n_cols + t - 1) / t); };
     if (g.M > 64) {
         if (tiles(256) >= 512) return launch_tile<256, 256, 2, 4, 2, OUT>(g, n_cols, st);
