@@ -998,6 +998,11 @@ template <int DT, class F> __device__ __forceinline__ void wide_each(const Choic
     }
 }
 
+// Blocks whose top-k fits well into the list: every class up to its bin is listed, and the rest is done there, so that no other
+// class needs its mass (256 x 50257 with top-k and top-p: 75.5 -> 60.4 us)
+__device__ __forceinline__ bool cuts_k(const Block& x) { return x.top_k > 0 && x.top_k < x.K; }
+__device__ __forceinline__ bool few_k(const Block& x) { return cuts_k(x) && x.top_k <= WIDE_LIST / 4; }
+
 template <int DT> __global__ void __launch_bounds__(WT) wide_top_kernel(Choice g, Wide w) {
     __shared__ int s_n;
     __shared__ TeamLds s_t;
@@ -1045,7 +1050,7 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_bins_kernel(Choice 
     s_t.count[t] = 0;
     __syncthreads();
     const int to = min(o.x.K, (c + 1) * w.chunk);
-    const bool mass = o.x.top_p < 1.0, count = o.x.top_k > 0;
+    const bool count = cuts_k(o.x), mass = o.x.top_p < 1.0 && !few_k(o.x);
     wide_each<DT>(g, o.x, c * w.chunk, to, [&](int, float v) {
         const float z = settle(v, o.inf);
         if (z > -INFINITY) {
@@ -1063,27 +1068,29 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_bins_kernel(Choice 
 // Which bins the edges fall into.  Top-k's is exact; the mass that top-k leaves is known up to its bin, so top-p's goal is one
 // of a range, and its bin too.
 struct Cut {
-    int k_bin;                                // bin of top-k's edge; WIDE_BINS: none
-    u64 k_before;                             // classes in the bins before it
+    int k_from, k_bin;                        // the bins that are listed for top-k, and the last one, its edge's; WIDE_BINS: none
+    u64 k_before;                             // classes in the bins before these
     u64 m_before, m_with;                     // mass in the bins before it, and with it
     int p_from, p_to;                         // bins that top-p's edge can fall into; p_from > p_to: none
     int sure;                                 // the bins before this one are kept
 };
 __device__ __forceinline__ Cut wide_cut(const Wide& w, const WideBlock& o, u64* s_mass, Cut* s_cut, TeamLds& s) {
     const int t = threadIdx.x;
-    const bool k = o.x.top_k > 0 && o.x.top_k < o.x.K, p = o.x.top_p < 1.0;
+    const bool k = cuts_k(o.x), few = few_k(o.x), p = o.x.top_p < 1.0 && !few;
     const u64 count = k ? o.s.count[t] : 0, mass = p ? o.s.mass[t] : 0;
     u64 total_count, total;
     const u64 crun = team_scan<WT>(count, s, total_count), mrun = team_scan<WT>(mass, s, total);
     s_mass[t] = mrun;
-    if (t == 0) *s_cut = Cut{WIDE_BINS, 0, total, total, 0, -1, WIDE_BINS};
+    // (fewer classes than top-k: all of them)
+    if (t == 0) *s_cut = few ? Cut{0, WIDE_BINS - 1, 0, 0, 0, 0, -1, 0} : Cut{WIDE_BINS, WIDE_BINS, 0, total, total, 0, -1, WIDE_BINS};
     __syncthreads();
     if (k && crun >= (u64)o.x.top_k && crun - count < (u64)o.x.top_k) {
         s_cut->k_bin = t;
-        s_cut->k_before = crun - count;
+        s_cut->k_from = few ? 0 : t;
+        s_cut->k_before = few ? 0 : crun - count;
         s_cut->m_before = mrun - mass;
         s_cut->m_with = mrun;
-        s_cut->sure = t;
+        s_cut->sure = few ? 0 : t;
     }
     __syncthreads();
     if (p) {
@@ -1101,7 +1108,7 @@ __device__ __forceinline__ Cut wide_cut(const Wide& w, const WideBlock& o, u64* 
 
 // Whether a chunk's kept mass follows from its bins: then `collect` takes no exponentials (they are most of its time: 64 x
 // 131071 23 us with them).  Not where min-p cuts inside a bin, nor for u = 0, which counts classes.
-__device__ __forceinline__ bool mass_is_binned(const Block& x) { return x.top_p < 1.0 && x.min_p == 0.0 && x.u > 0.0; }
+__device__ __forceinline__ bool mass_is_binned(const Block& x) { return x.top_p < 1.0 && x.min_p == 0.0 && x.u > 0.0 && !few_k(x); }
 
 template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choice g, Wide w) {
     __shared__ int s_n;
@@ -1124,7 +1131,7 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choi
         const float z = settle(v, o.inf);
         if (!(z > -INFINITY)) return;
         const int bin = wide_bin(o, z);
-        if (bin == cut.k_bin || (bin >= cut.p_from && bin <= cut.p_to)) {
+        if ((bin >= cut.k_from && bin <= cut.k_bin) || (bin >= cut.p_from && bin <= cut.p_to)) {
             const unsigned at = atomicAdd(&s_listed, 1u);
             const u64 place = place_of(key_of(z), (unsigned)i);
             if (at < 1024) s_list[at] = place;
@@ -1253,18 +1260,26 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_finish_kernel(Choic
     auto weight = [&](u64 place) { return units(mass_of(z_of(place), o.top, o.x.c), o.scale); };
     u64 edge = 0;
     u64 k_mass = cut.m_before;
+    const bool few = few_k(o.x);
     if (cut.k_bin < WIDE_BINS) {
-        edge = list_edge(s_list, n, (double)o.x.top_k, cut.k_before, s_t, [&](u64 p) { return wide_bin(o, z_of(p)) == cut.k_bin; },
-                         [](u64) { return (u64)1; });
-        if (cut.p_from <= cut.p_to) {
+        edge = list_edge(s_list, n, (double)o.x.top_k, cut.k_before, s_t, [&](u64 p) {
+            const int bin = wide_bin(o, z_of(p));
+            return bin >= cut.k_from && bin <= cut.k_bin;
+        }, [](u64) { return (u64)1; });
+        if (cut.p_from <= cut.p_to || few) {
             u64 own = 0, sum;
-            for (int i = t; i < n; i += WT)
-                if (wide_bin(o, z_of(s_list[i])) == cut.k_bin && s_list[i] >= edge) own += weight(s_list[i]);
+            for (int i = t; i < n; i += WT) {
+                const int bin = wide_bin(o, z_of(s_list[i]));
+                if (bin >= cut.k_from && bin <= cut.k_bin && s_list[i] >= edge) own += weight(s_list[i]);
+            }
             team_scan<WT>(own, s_t, sum);
-            k_mass += sum;
+            k_mass = few ? sum : k_mass + sum;
         }
     }
-    if (cut.p_from <= cut.p_to) {
+    if (few && o.x.top_p < 1.0) {
+        const u64 least = edge;
+        edge = max(edge, list_edge(s_list, n, o.x.top_p * (double)k_mass, 0, s_t, [&](u64 p) { return p >= least; }, weight));
+    } else if (cut.p_from <= cut.p_to) {
         const u64 least = edge;
         const u64 to = list_edge(s_list, n, o.x.top_p * (double)k_mass, cut.p_from ? s_mass[cut.p_from - 1] : 0, s_t, [&](u64 p) {
             const int bin = wide_bin(o, z_of(p));

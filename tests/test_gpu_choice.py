@@ -349,3 +349,16 @@ def test_offsets_that_pass_32_bits():
         a = ops.sample_categories(far, u, offsets(classes), log_prob=True, **p)
         b = ops.sample_categories(z.to(DEV), u, offsets(classes), log_prob=True, **p)
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("left", [2, 10, 64, 65, 200, 1500])
+def test_fewer_classes_left_than_top_k(left):
+    K = 5000
+    z = torch.full((4, K), -math.inf)
+    g = torch.Generator().manual_seed(left)
+    for b in range(4):
+        z[b, torch.randperm(K, generator=g)[:left]] = 2 * torch.randn((left,), generator=g)
+    for k in (left - 1, left, left + 1, 1024, 1025, 3000):
+        for p in ({"top_k": k}, {"top_k": k, "top_p": 0.6}, {"top_k": k, "top_p": 0.9, "min_p": 0.05}):
+            check(z, uniforms(4, 1, left), [K], **p)
+            check(z, torch.zeros(4, 1), [K], **p)
