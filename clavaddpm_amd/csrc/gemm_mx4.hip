@@ -178,10 +178,11 @@ __global__ void __launch_bounds__(WN * WM * 64) mx4_tile_kernel(Mx4Args g, int t
     // workgroups go round robin over the 8 XCDs: each takes a run of tiles, for its L2
     const int xcd = (int)blockIdx.x & 7, per = tiles >> 3, rem = tiles & 7;
     const int tile = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + ((int)blockIdx.x >> 3);
-    // in it, eight tiles down before the next column: the 32 tiles that an XCD works on at a time then share 8 panels of X and 4
-    // of W (a row of tiles: 1 and 32)
-    const int tiles_m = tiles / tiles_n, group = tile / (8 * tiles_n), gm = min(8, tiles_m - 8 * group), in = tile - group * 8 * tiles_n;
-    const int m0 = (8 * group + in % gm) * BM, n0 = in / gm * BN;
+    // in it, DOWN tiles down before the next column: the 32 tiles that an XCD works on at a time then share 6 panels of X and 5
+    // or 6 of W (a row of tiles: 1 and 32; 16384 x 8192 x 8192 to bfloat16, six down 546 us, four 544, eight 573, sixteen 576)
+    constexpr int DOWN = 6;
+    const int tiles_m = tiles / tiles_n, group = tile / (DOWN * tiles_n), gm = min(DOWN, tiles_m - DOWN * group), in = tile - group * DOWN * tiles_n;
+    const int m0 = (DOWN * group + in % gm) * BM, n0 = in / gm * BN;
 
     // LDS row `row` of W holds the column of y that puts the 16 accumulators of a lane side by side: its half h of a 32 x 32
     // product has rows 8 G + 4 h + t, G, t < 4, and they are to be columns 16 h + 4 G + t.  Sources are a base of the tile (in scalar registers) and 32 bits of a lane's own.
@@ -316,6 +317,14 @@ __global__ void __launch_bounds__(WN * WM * 64) mx4_tile_kernel(Mx4Args g, int t
     // lines (4096 x 1024 x 1024 to float32: 13.5 -> 10.6 us).
     constexpr int SZ = OUT == CLAVA_DT_F32 ? 4 : 2, TILES = SZ == 2 && TN % 2 == 0 ? 2 : 1, ROW = 32 * TILES * SZ, PITCH = ROW + 16, PER = ROW / 16;
     static_assert(NW * 32 * PITCH <= NS * STAGE, "the strips fit into the stages");
+    // Results of the largest tiles go past the caches, which they would take from the panels: 16384 x 8192 x 8192 540 -> 518 us,
+    // with the pack that reads it 606 -> 580.  Smaller results are still there for their reader, which is worth as much (20000 x
+    // 1024 x 512 to bfloat16, kept / past: 15.1 / 14.4 us, with the pack 23.3 / 24.2).
+    constexpr bool PAST = BN == 256 && BM == 256;
+    auto put = [](auto u, auto* to) {
+        if (PAST) __builtin_nontemporal_store(u, to);
+        else *to = u;
+    };
     char* const strip = smem + wave * 32 * PITCH;
 #pragma unroll
     for (int i = 0; i < TN; i += TILES) {
@@ -359,8 +368,8 @@ __global__ void __launch_bounds__(WN * WM * 64) mx4_tile_kernel(Mx4Args g, int t
                 if (m >= g.M || n >= g.N) continue;
                 char* const to = static_cast<char*>(g.y) + ((size_t)m * g.ldy + n) * SZ;
                 if (n + 16 / SZ <= g.N) {
-                    if (SZ == 4) *reinterpret_cast<u32x4_u4*>(to) = u;
-                    else *reinterpret_cast<u32x4_u2*>(to) = u;
+                    if (SZ == 4) put(u, reinterpret_cast<u32x4_u4*>(to));
+                    else put(u, reinterpret_cast<u32x4_u2*>(to));
                 } else {
 #pragma unroll
                     for (int e = 0; e < 16 / SZ; ++e)
