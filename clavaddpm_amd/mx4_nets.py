@@ -4,6 +4,8 @@ The stack is MLPDiffusion's proj + mlp (`tab_ddpm/modules.py:425-460`).  proj an
 columns and the time embedding, and write the noise estimate and the logits - and hold a few per cent of the work; the
 hidden blocks' weights are packed once per chain, and every block writes the next one's packed operand itself.  4 bits keep
 about one decimal digit per activation: samples differ visibly from the float32 ones, which the split-f16 mode reproduces.
+The kernel of a layer, and with it the order of a row's sums, follows from the number of rows (up to 16, up to 64, more): a last
+bit of difference there can move a 4-bit rounding of the next layer, so batches of such different sizes can differ in single values.
 """
 from . import _lib, ops
 
