@@ -5,6 +5,7 @@ caching allocator, and the raw-pointer call.  All arithmetic is in the HIP
 library.
 """
 import ctypes
+import functools
 import math
 
 import torch
@@ -354,7 +355,7 @@ def _same_device(dev, **tensors):
 def _launch(dev, name, f, *args):
     """f(*args, stream) on the current stream of the tensors' device."""
     index = dev.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
@@ -526,6 +527,7 @@ class _CChoice(ctypes.Structure):
 
 
 _CHOICE_RANGE = {"temperature": (0.0, math.inf), "top_p": (0.0, math.inf), "min_p": (0.0, 1.0), "top_k": (-2 ** 63, 2 ** 63)}
+_NUMBERS = {int, float}
 
 
 def _choice_args(dev, rows, features, values):
@@ -550,6 +552,12 @@ def _choice_args(dev, rows, features, values):
             _refuse(f"sample_categories: {name} {v}, expected {'a whole number' if name == 'top_k' else f'in [{low}, {high}]'}")
         setattr(c, name, max(-1, min(int(v), 2 ** 31 - 1)) if name == "top_k" else v)
     return c
+
+
+@functools.lru_cache(maxsize=64)
+def _choice_numbers(*values):
+    """The struct of four numbers, which C only reads (building it takes 2 of a small call's 11 us)."""
+    return _choice_args(None, 0, 0, zip(_CHOICE_RANGE, values))
 
 
 def sample_categories(logits, uniforms=None, offsets=None, max_classes=None, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -590,7 +598,8 @@ def sample_categories(logits, uniforms=None, offsets=None, max_classes=None, *, 
         out = torch.empty((B, m), device=dev, dtype=torch.int32)
     elif out.dtype is not torch.int32 or out.shape != (B, m) or not out.is_contiguous() or out.device != dev:
         _refuse(f"sample_categories: out must be contiguous int32 [{B},{m}] on {dev}")
-    c = _choice_args(dev, B, m, (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)))
+    values = temperature, top_p, min_p, top_k
+    c = _choice_numbers(*values) if _NUMBERS.issuperset(map(type, values)) else _choice_args(dev, B, m, zip(_CHOICE_RANGE, values))
     lp = torch.empty((B, m), device=dev, dtype=torch.float32) if log_prob else None
     need, ws = 0, None
     if max_classes > 2048:
