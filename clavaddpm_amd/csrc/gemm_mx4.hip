@@ -320,10 +320,10 @@ __global__ void __launch_bounds__(WN * WM * 64) mx4_tile_kernel(Mx4Args g, int t
     // lines (4096 x 1024 x 1024 to float32: 13.5 -> 10.6 us).
     constexpr int SZ = OUT == CLAVA_DT_F32 ? 4 : 2, TILES = SZ == 2 && TN % 2 == 0 ? 2 : 1, ROW = 32 * TILES * SZ, PITCH = ROW + 16, PER = ROW / 16;
     static_assert(NW * 32 * PITCH <= NS * STAGE, "the strips fit into the stages");
-    // Results of the largest tiles go past the caches, which they would take from the panels: 16384 x 8192 x 8192 540 -> 518 us,
-    // with the pack that reads it 606 -> 580.  Smaller results are still there for their reader, which is worth as much (20000 x
-    // 1024 x 512 to bfloat16, kept / past: 15.1 / 14.4 us, with the pack 23.3 / 24.2).
-    constexpr bool PAST = BN == 256 && BM == 256;
+    // Results of many tiles go past the caches, which they would take from the panels: 16384 x 8192 x 8192 540 -> 518 us, with the
+    // pack that reads it 606 -> 580; 20000 x 1024 x 512 to bfloat16 15.1 -> 14.4, with it 23.3 -> 24.2; 4096 x 1024 x 1024 to float32
+    // 9.5 -> 8.0, with it 18.1 -> 17.4.  Those of 64 x 64 tiles are small and stay for their reader.
+    constexpr bool PAST = BN >= 128;
     auto put = [](auto u, auto* to) {
         if (PAST) __builtin_nontemporal_store(u, to);
         else *to = u;
