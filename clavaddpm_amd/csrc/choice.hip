@@ -890,9 +890,9 @@ template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64
 
 // ------------------------------------------------------------------------------------------- very many classes, in chunks
 // Four launches over chunks of a block (top -> bins -> collect) and over blocks (finish).  Weights are integers, so that the
-// sums over chunks have no order.  64 x 131071 bfloat16 with top-p: 6.8 + 18.8 + 17.6 + 17.6 us; reading it once takes 3.6.  The
+// sums over chunks have no order.  64 x 131071 bfloat16 with top-p: 6.6 + 17.8 + 15.3 + 17.0 us; reading it once takes 3.6.  The
 // second is bound by its masses (8.4 million float64 exponentials), the others by the latency of a few dependent loads and
-// workgroup sums; so are all four of 1 x 262144 with top-k (3.2 + 7.6 + 7.0 + 9.7).  Between the launches, for every wide block
+// workgroup sums; so are all four of 1 x 262144 with top-k (3.0 + 7.6 + 6.3 + 9.9).  Between the launches, for every wide block
 // and in `ws`:
 constexpr int WT = 256, WIDE_BINS = 256, WIDE_LIST = 4096, WIDE_CHUNKS = 1024;
 struct Wide {
@@ -956,8 +956,7 @@ struct WideBlock {
     double scale;
     float inv;
 };
-// Block and, from the chunks' ranges on (`ranges`), what they say of it
-__device__ __forceinline__ bool wide_block(const Choice& g, const Wide& w, long long block, bool ranges, WideBlock& o, int* s_n, TeamLds& t) {
+__device__ __forceinline__ bool wide_block(const Choice& g, const Wide& w, long long block, WideBlock& o, int* s_n) {
     const int b = (int)(block / w.per_row);
     const int f = wide_feature(g, (int)(block - (long long)b * w.per_row), s_n);
     if (f < 0) return false;
@@ -965,45 +964,22 @@ __device__ __forceinline__ bool wide_block(const Choice& g, const Wide& w, long 
     o.s = wide_ws(w, block);
     o.chunks = (o.x.K + w.chunk - 1) / w.chunk;
     o.scale = unit_scale(o.x.K);
-    if (!ranges) return true;
-    float top = -INFINITY, bottom = INFINITY;
-    u64 bad = 0, nan;
-    for (int i = threadIdx.x; i < o.chunks; i += WT) {
-        const float hi = o.s.range[2 * i], lo = o.s.range[2 * i + 1];
-        bad += hi != hi;
-        top = fmaxf(top, hi);
-        bottom = fminf(bottom, lo);
-    }
-    team_scan<WT>(bad, t, nan);
-    top = group_max<64>(top);
-    bottom = -group_max<64>(-bottom);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) t.part[threadIdx.x >> 6] = (u64)__float_as_uint(top) << 32 | __float_as_uint(bottom);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < WT / 64; ++i) {
-        top = fmaxf(top, __uint_as_float((unsigned)(t.part[i] >> 32)));
-        bottom = fminf(bottom, __uint_as_float((unsigned)t.part[i]));
-    }
-    o.inf = top == INFINITY;
-    o.top = o.inf ? 0.f : top;
-    o.none = nan || o.x.bad || top == -INFINITY;
-    o.inv = bins_per_unit(top, bottom, o.x.T, (float)WIDE_BINS);
     return true;
 }
 __device__ __forceinline__ int wide_bin(const WideBlock& o, float z) {
     return linear_bin(z, o.top, o.inv, WIDE_BINS);
 }
 
-// f(class, logit) for the classes from .. to, eight neighbouring ones a thread
+// f(first class, logits) for the classes from .. to, eight neighbouring ones a thread; -inf where there are fewer
 template <int DT, class F> __device__ __forceinline__ void wide_each(const Choice& g, const Block& x, int from, int to, F f) {
     for (int i = from + (int)threadIdx.x * 8; i < to; i += WT * 8) {
         float z[8];
         const int n = to - i;
         load8<DT>(g.z, x.at + i, n, z);
+        if (n < 8)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < n) f(i + j, z[j]);
+            for (int j = 0; j < 8; ++j) z[j] = j < n ? z[j] : -INFINITY;
+        f(i, z);
     }
 }
 
@@ -1012,11 +988,91 @@ template <int DT, class F> __device__ __forceinline__ void wide_each(const Choic
 __device__ __forceinline__ bool cuts_k(const Block& x) { return x.top_k > 0 && x.top_k < x.K; }
 __device__ __forceinline__ bool few_k(const Block& x) { return cuts_k(x) && x.top_k <= WIDE_LIST / 4; }
 
+// Which bins the edges fall into.  Top-k's is exact; the mass that top-k leaves is known up to its bin, so top-p's goal is one
+// of a range, and its bin too.
+struct Cut {
+    int k_from, k_bin;                        // the bins that are listed for top-k, and the last one, its edge's; WIDE_BINS: none
+    u64 k_before;                             // classes in the bins before these
+    u64 m_before;                             // mass in the bins before top-k's; without one all of it
+    int p_from, p_to;                         // bins that top-p's edge can fall into; p_from > p_to: none
+    int sure;                                 // the bins before this one are kept
+};
+// What every workgroup of a block has to know of it before it starts.  One wavefront finds it, four bins a lane, and the
+// others wait at one barrier (with scans over the workgroup instead, and a barrier or two for each, `collect` took 18.4 us for 17.0).
+struct WideHead {
+    float top, bottom;
+    int nan;
+    Cut cut;
+};
+template <bool CUT> __device__ __forceinline__ void wide_head(const WideBlock& o, WideHead& h, u64* s_mass) {
+    if (threadIdx.x >= 64) return;
+    const int lane = threadIdx.x;
+    const bool k = CUT && cuts_k(o.x), few = CUT && few_k(o.x), p = CUT && o.x.top_p < 1.0 && !few;
+    u64 count[4], mass[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        count[i] = k ? o.s.count[4 * lane + i] : 0;
+        mass[i] = p ? o.s.mass[4 * lane + i] : 0;
+    }
+    float top = -INFINITY, bottom = INFINITY;
+    bool nan = false;
+    for (int i = lane; i < o.chunks; i += 64) {
+        const float hi = o.s.range[2 * i], lo = o.s.range[2 * i + 1];
+        nan |= hi != hi;
+        top = fmaxf(top, hi);
+        bottom = fminf(bottom, lo);
+    }
+    top = group_max<64>(top);
+    bottom = -group_max<64>(-bottom);
+    nan = __any(nan);
+    Cut c = {WIDE_BINS, WIDE_BINS, 0, 0, 0, -1, WIDE_BINS};
+    if (CUT) {
+        // running sums, up to and with each bin of the lane
+#pragma unroll
+        for (int i = 1; i < 4; ++i) { count[i] += count[i - 1]; mass[i] += mass[i - 1]; }
+        const u64 c0 = scan<64>(count[3]) - count[3], m0 = scan<64>(mass[3]) - mass[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { count[i] += c0; mass[i] += m0; }
+        const u64 total = at_lane(mass[3], 63);
+        if (s_mass)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_mass[4 * lane + i] = mass[i];
+        // the first bin whose running sum reaches a goal, and the sum before it and with it
+        auto value = [](const u64* v, int i) { return i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3]; };
+        auto first = [&](const u64* v, double goal) {
+            const u64 past = __ballot((double)v[3] >= goal);
+            const int i = ((double)v[0] < goal) + ((double)v[1] < goal) + ((double)v[2] < goal), at = past ? (int)__builtin_ctzll(past) : 0;
+            return past ? 4 * at + at_lane(i, at) : -1;
+        };
+        auto upto = [&](const u64* v, int bin) { return bin < 0 ? (u64)0 : at_lane(value(v, bin & 3), bin >> 2); };
+        u64 m_with = total;
+        c.m_before = total;
+        const int bin = k ? first(count, (double)o.x.top_k) : -1;
+        if (few) c = Cut{0, bin < 0 ? WIDE_BINS - 1 : bin, 0, 0, 0, -1, 0};      // (fewer classes than top-k: all of them)
+        else if (bin >= 0) {
+            m_with = upto(mass, bin);
+            c = Cut{bin, bin, upto(count, bin - 1), upto(mass, bin - 1), 0, -1, bin};
+        }
+        if (p) {
+            c.p_from = first(mass, o.x.top_p * (double)c.m_before);
+            c.p_to = first(mass, o.x.top_p * (double)m_with);
+            c.sure = min(c.sure, c.p_from);
+        }
+    }
+    if (lane == 0) h = WideHead{top, bottom, nan, c};
+}
+__device__ __forceinline__ void wide_look(WideBlock& o, const WideHead& h) {
+    o.inf = h.top == INFINITY;
+    o.top = o.inf ? 0.f : h.top;
+    o.none = h.nan || o.x.bad || h.top == -INFINITY;
+    o.inv = bins_per_unit(h.top, h.bottom, o.x.T, (float)WIDE_BINS);
+}
+
 template <int DT> __global__ void __launch_bounds__(WT) wide_top_kernel(Choice g, Wide w) {
     __shared__ int s_n;
     __shared__ TeamLds s_t;
     WideBlock o;
-    if (!wide_block(g, w, blockIdx.y, false, o, &s_n, s_t)) return;
+    if (!wide_block(g, w, blockIdx.y, o, &s_n)) return;
     const int c = blockIdx.x, t = threadIdx.x;
     if (c == 0 && (w.k || w.p)) {
         if (t == 0) *o.s.listed = 0;
@@ -1027,10 +1083,13 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_top_kernel(Choice g
     float top = -INFINITY, bottom = INFINITY;
     bool nan = false;
     const int to = min(o.x.K, (c + 1) * w.chunk);
-    wide_each<DT>(g, o.x, c * w.chunk, to, [&](int, float z) {
-        nan |= z != z;
-        top = fmaxf(top, z);
-        bottom = z == -INFINITY ? bottom : fminf(bottom, z);
+    wide_each<DT>(g, o.x, c * w.chunk, to, [&](int, const float* z) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            nan |= z[j] != z[j];
+            top = fmaxf(top, z[j]);
+            bottom = z[j] == -INFINITY ? bottom : fminf(bottom, z[j]);
+        }
     });
     top = group_max<64>(top);
     bottom = -group_max<64>(-bottom);
@@ -1051,21 +1110,28 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_top_kernel(Choice g
 template <int DT> __global__ void __launch_bounds__(WT) wide_bins_kernel(Choice g, Wide w) {
     __shared__ int s_n;
     __shared__ TeamLds s_t;
+    __shared__ WideHead s_head;
     WideBlock o;
-    if (!wide_block(g, w, blockIdx.y, true, o, &s_n, s_t)) return;
+    if (!wide_block(g, w, blockIdx.y, o, &s_n)) return;
     const int c = blockIdx.x, t = threadIdx.x;
-    if (c >= o.chunks || o.none) return;
+    if (c >= o.chunks) return;
     s_t.weight[t] = 0;
     s_t.count[t] = 0;
+    wide_head<false>(o, s_head, nullptr);
     __syncthreads();
+    wide_look(o, s_head);
+    if (o.none) return;
     const int to = min(o.x.K, (c + 1) * w.chunk);
     const bool count = cuts_k(o.x), mass = o.x.top_p < 1.0 && !few_k(o.x);
-    wide_each<DT>(g, o.x, c * w.chunk, to, [&](int, float v) {
-        const float z = settle(v, o.inf);
-        if (z > -INFINITY) {
-            const int bin = wide_bin(o, z);
-            if (mass) atomicAdd(&s_t.weight[bin], units(mass_of(z, o.top, o.x.c), o.scale));
-            if (count) atomicAdd(&s_t.count[bin], 1u);
+    wide_each<DT>(g, o.x, c * w.chunk, to, [&](int, const float* v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float z = settle(v[j], o.inf);
+            if (z > -INFINITY) {
+                const int bin = wide_bin(o, z);
+                if (mass) atomicAdd(&s_t.weight[bin], units(mass_of(z, o.top, o.x.c), o.scale));
+                if (count) atomicAdd(&s_t.count[bin], 1u);
+            }
         }
     });
     __syncthreads();
@@ -1074,95 +1140,75 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_bins_kernel(Choice 
     if (s_t.count[t]) atomicAdd(&o.s.count[t], s_t.count[t]);
 }
 
-// Which bins the edges fall into.  Top-k's is exact; the mass that top-k leaves is known up to its bin, so top-p's goal is one
-// of a range, and its bin too.
-struct Cut {
-    int k_from, k_bin;                        // the bins that are listed for top-k, and the last one, its edge's; WIDE_BINS: none
-    u64 k_before;                             // classes in the bins before these
-    u64 m_before, m_with;                     // mass in the bins before it, and with it
-    int p_from, p_to;                         // bins that top-p's edge can fall into; p_from > p_to: none
-    int sure;                                 // the bins before this one are kept
-};
-__device__ __forceinline__ Cut wide_cut(const Wide& w, const WideBlock& o, u64* s_mass, Cut* s_cut, TeamLds& s) {
-    const int t = threadIdx.x;
-    const bool k = cuts_k(o.x), few = few_k(o.x), p = o.x.top_p < 1.0 && !few;
-    const u64 count = k ? o.s.count[t] : 0, mass = p ? o.s.mass[t] : 0;
-    u64 total_count, total;
-    const u64 crun = team_scan<WT>(count, s, total_count), mrun = team_scan<WT>(mass, s, total);
-    s_mass[t] = mrun;
-    // (fewer classes than top-k: all of them)
-    if (t == 0) *s_cut = few ? Cut{0, WIDE_BINS - 1, 0, 0, 0, 0, -1, 0} : Cut{WIDE_BINS, WIDE_BINS, 0, total, total, 0, -1, WIDE_BINS};
-    __syncthreads();
-    if (k && crun >= (u64)o.x.top_k && crun - count < (u64)o.x.top_k) {
-        s_cut->k_bin = t;
-        s_cut->k_from = few ? 0 : t;
-        s_cut->k_before = few ? 0 : crun - count;
-        s_cut->m_before = mrun - mass;
-        s_cut->m_with = mrun;
-        s_cut->sure = few ? 0 : t;
-    }
-    __syncthreads();
-    if (p) {
-        const double lo = o.x.top_p * (double)s_cut->m_before, hi = o.x.top_p * (double)s_cut->m_with;
-        const double before = (double)(mrun - mass), with = (double)mrun;
-        // the first bin at which the running mass reaches each end of the goal's range
-        if (with >= lo && (t == 0 || before < lo)) { s_cut->p_from = t; }
-        if (with >= hi && (t == 0 || before < hi)) { s_cut->p_to = t; }
-    }
-    __syncthreads();
-    Cut c = *s_cut;
-    if (p) c.sure = min(c.sure, c.p_from);
-    return c;
-}
-
-// Whether a chunk's kept mass follows from its bins: then `collect` takes no exponentials (they are most of its time: 64 x
-// 131071 23 us with them).  Not where min-p cuts inside a bin, nor for u = 0, which counts classes.
+// Whether a chunk's kept mass follows from its bins: then `collect` takes no exponentials (64 x 131071: 23 us with
+// them, 18 without).  Not where min-p cuts inside a bin, nor for u = 0, which counts classes.
 __device__ __forceinline__ bool mass_is_binned(const Block& x) { return x.top_p < 1.0 && x.min_p == 0.0 && x.u > 0.0 && !few_k(x); }
 
 template <int DT> __global__ void __launch_bounds__(WT) wide_collect_kernel(Choice g, Wide w) {
     __shared__ int s_n;
-    __shared__ TeamLds s_t;
-    __shared__ u64 s_mass[WIDE_BINS];
-    __shared__ Cut s_cut;
-    __shared__ u64 s_list[1024];
+    __shared__ WideHead s_head;
+    __shared__ u64 s_list[1024], s_sum, s_any;
     __shared__ unsigned s_listed, s_base;
     WideBlock o;
-    if (!wide_block(g, w, blockIdx.y, true, o, &s_n, s_t)) return;
+    if (!wide_block(g, w, blockIdx.y, o, &s_n)) return;
     const int c = blockIdx.x, t = threadIdx.x;
-    if (c >= o.chunks || o.none) return;
-    const Cut cut = wide_cut(w, o, s_mass, &s_cut, s_t);
-    if (t == 0) s_listed = 0;
-    __syncthreads();
-    const int to = min(o.x.K, (c + 1) * w.chunk);
+    if (c >= o.chunks) return;
+    if (t == 0) { s_listed = 0; s_sum = 0; s_any = 0; }
     const bool binned = mass_is_binned(o.x);
+    const u64 chunk_mass = binned ? o.s.chunk_mass[c * WIDE_BINS + t] : 0;
+    wide_head<true>(o, s_head, nullptr);
+    __syncthreads();
+    wide_look(o, s_head);
+    if (o.none) return;
+    const Cut cut = s_head.cut;
+    const int to = min(o.x.K, (c + 1) * w.chunk);
     u64 sum = 0, any = 0;
-    wide_each<DT>(g, o.x, c * w.chunk, to, [&](int i, float v) {
-        const float z = settle(v, o.inf);
-        if (!(z > -INFINITY)) return;
-        const int bin = wide_bin(o, z);
-        if ((bin >= cut.k_from && bin <= cut.k_bin) || (bin >= cut.p_from && bin <= cut.p_to)) {
-            const unsigned at = atomicAdd(&s_listed, 1u);
-            const u64 place = place_of(key_of(z), (unsigned)i);
-            if (at < 1024) s_list[at] = place;
-            else {                                            // more than a chunk usually has
-                const unsigned far = atomicAdd(o.s.listed, 1u);
-                if (far < WIDE_LIST) o.s.list[far] = place;
+    // (a class's bin is not cut to an integer here: it is compared with the ends of the listed ones)
+    const float k_from = (float)cut.k_from, k_end = (float)(cut.k_bin + 1), p_from = (float)cut.p_from, p_end = (float)(cut.p_to + 1),
+                sure = (float)cut.sure;
+    wide_each<DT>(g, o.x, c * w.chunk, to, [&](int i, const float* v) {
+        unsigned which = 0;
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            z[j] = settle(v[j], o.inf);
+            const float bin = z[j] == -INFINITY ? INFINITY : o.inv > 0.f ? fminf((o.top - z[j]) * o.inv, (float)(WIDE_BINS - 1)) : 0.f;
+            const bool is = (bin >= k_from && bin < k_end) || (bin >= p_from && bin < p_end);
+            which |= is ? 1u << j : 0u;
+            if (!binned && !is && bin < sure) {
+                const double a = mass_of(z[j], o.top, o.x.c);
+                if (a >= o.x.min_p) { sum += units(a, o.scale); any += a > 0.0; }
             }
-        } else if (bin < cut.sure && !binned) {
-            const double a = mass_of(z, o.top, o.x.c);
-            if (a >= o.x.min_p) { sum += units(a, o.scale); any += a > 0.0; }
         }
+        if (which == 0) return;
+        unsigned at = atomicAdd(&s_listed, (unsigned)__popc(which));
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (which >> j & 1) {
+                const u64 place = place_of(key_of(z[j]), (unsigned)(i + j));
+                if (at < 1024) s_list[at] = place;
+                else {                                        // more than a chunk usually has
+                    const unsigned far = atomicAdd(o.s.listed, 1u);
+                    if (far < WIDE_LIST) o.s.list[far] = place;
+                }
+                ++at;
+            }
     });
-    u64 total, n_any;
-    if (binned) sum = t < cut.sure ? o.s.chunk_mass[c * WIDE_BINS + t] : 0;
-    team_scan<WT>(sum, s_t, total);
-    team_scan<WT>(any, s_t, n_any);
+    if (binned) sum = t < cut.sure ? chunk_mass : 0;
+    sum = scan<64>(sum);
+    if ((t & 63) == 63 && sum) atomicAdd(&s_sum, sum);
+    if (o.x.u == 0.0) {
+        any = scan<64>(any);
+        if ((t & 63) == 63 && any) atomicAdd(&s_any, any);
+    }
+    __syncthreads();
     const unsigned n = min(s_listed, 1024u);
     if (t == 0) {
-        o.s.sum[c] = total;
-        o.s.any[c] = (unsigned)n_any;
-        s_base = n ? atomicAdd(o.s.listed, n) : 0;
+        o.s.sum[c] = s_sum;
+        o.s.any[c] = (unsigned)s_any;
+        if (n) s_base = atomicAdd(o.s.listed, n);
     }
+    if (n == 0) return;
     __syncthreads();
     for (unsigned i = t; i < n; i += WT)
         if (s_base + i < WIDE_LIST) o.s.list[s_base + i] = s_list[i];
@@ -1241,19 +1287,22 @@ template <int DT> __global__ void __launch_bounds__(WT) wide_finish_kernel(Choic
     __shared__ int s_n;
     __shared__ TeamLds s_t;
     __shared__ u64 s_mass[WIDE_BINS];
-    __shared__ Cut s_cut;
+    __shared__ WideHead s_head;
     __shared__ u64 s_sum[WIDE_CHUNKS];
     __shared__ u64 s_list[WIDE_LIST];
     __shared__ int s_chunk;
     __shared__ u64 s_before;
     WideBlock o;
-    if (!wide_block(g, w, blockIdx.x, true, o, &s_n, s_t)) return;
+    if (!wide_block(g, w, blockIdx.x, o, &s_n)) return;
     const int t = threadIdx.x;
+    wide_head<true>(o, s_head, s_mass);
+    __syncthreads();
+    wide_look(o, s_head);
     if (o.none) {
         if (t == 0) give(g, o.x.b, o.x.f, -1, no_number());
         return;
     }
-    const Cut cut = wide_cut(w, o, s_mass, &s_cut, s_t);
+    const Cut cut = s_head.cut;
     const unsigned listed = w.k || w.p ? *o.s.listed : 0;
     if (listed > WIDE_LIST) {                                 // too many classes in the edges' bins
         choose_team<WT, DT>(g, o.x, s_t);
