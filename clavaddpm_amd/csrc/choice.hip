@@ -74,9 +74,11 @@ __device__ __forceinline__ double exp2_nonpos(double y) {
     y = fmax(y, -1100.0);
     const double n = rint(y), r = y - n;
     double p = c.t[11];
+    // (written out, since the terms belong in scalar registers: the compiler kept 22 vector registers of them and copied one for
+    // every step)
 #pragma unroll
-    for (int k = 10; k >= 0; --k) p = fma(p, r, c.t[k]);
-    return ldexp(p, (int)n);
+    for (int k = 10; k >= 1; --k) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p) : "v"(p), "v"(r), "s"(c.t[k]));
+    return ldexp(fma(p, r, 1.0), (int)n);
 }
 // log(x) for x >= 1: the float32 logarithm and one Newton step on e^y = x (its square, 1e-14, is what stays)
 __device__ __forceinline__ double log_from1(double x) {
@@ -154,16 +156,15 @@ __device__ __forceinline__ void give(const Choice& g, int b, int f, int idx, flo
 __device__ __forceinline__ float no_number() { return __uint_as_float(0x7fc00000u); }
 
 // ------------------------------------------------------------------------------------------------------ lanes of a group
-template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ double dpp_d(double v) {      // 0 where there is no source lane
-    const u64 b = (u64)__double_as_longlong(v);
-    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
-    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
-    return __longlong_as_double((long long)((u64)hi << 32 | lo));
+// The value of the lane that CTRL names, 0 where there is none or the row is not in ROWS
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ unsigned dpp_d(unsigned b) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, ROWS == 0xf);
 }
 template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ u64 dpp_d(u64 b) {
-    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
-    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
-    return (u64)hi << 32 | lo;
+    return (u64)dpp_d<CTRL, ROWS>((unsigned)(b >> 32)) << 32 | dpp_d<CTRL, ROWS>((unsigned)b);
+}
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ double dpp_d(double v) {
+    return __longlong_as_double((long long)dpp_d<CTRL, ROWS>((u64)__double_as_longlong(v)));
 }
 // The lane, computed anew: what follows from it (a lane mask for every step of a sort) is not kept over a loop of blocks,
 // where it took 240 scalar registers
@@ -171,9 +172,6 @@ __device__ __forceinline__ int lane_here() {
     int l = threadIdx.x & 63;
     asm volatile("" : "+v"(l));
     return l;
-}
-template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ unsigned dpp_d(unsigned b) {
-    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
 }
 // Inclusive sums in lane order within groups of G lanes
 template <int G, class T> __device__ __forceinline__ T scan(T v) {
