@@ -14,8 +14,9 @@
 // block in LDS; wider ones are cut into chunks over many workgroups and joined (wide_*).
 //
 // Each logit is read once up to 2048 classes (wider: three or four times, from the caches mostly), so that memory would need
-// 30 us for 4096 rows of 50 features with 8.1k classes (float32).  They take 126 us, all filters at 20000 rows 855 (145): bound
-// by vector instructions, 304 and 379 a block, most of them float64 - a mass takes 20.
+// 30 us for 4096 rows of 50 features with 8.1k classes (float32).  They take 115 us, all filters at 20000 rows 768 (145): bound
+// by vector instructions, 254 and 373 a block, three quarters and four fifths of the issue cycles, most of them float64 - a
+// mass takes 20.
 #include "elem.h"
 #include "rng.h"
 #include "wave.h"
@@ -75,7 +76,7 @@ __device__ __forceinline__ double exp2_nonpos(double y) {
     const double n = rint(y), r = y - n;
     double p = c.t[11];
     // (written out, since the terms belong in scalar registers: the compiler kept 22 vector registers of them and copied one for
-    // every step)
+    // every step; 20000 x 50 filtered 884 -> 795 us together with lane moves that need no zero first)
 #pragma unroll
     for (int k = 10; k >= 1; --k) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p) : "v"(p), "v"(r), "s"(c.t[k]));
     return ldexp(fma(p, r, 1.0), (int)n);
@@ -827,7 +828,8 @@ __device__ __forceinline__ unsigned choose_narrow(const Choice& g, const int* pe
 }
 
 // A wavefront takes blocks of one width class after another: narrow ones share it, others have it to themselves.  Five of them a
-// SIMD (NV = 16): the waits of one are the others' work (20000 x 50 filtered, four / five / six: 1111 / 960 / 1088 us, six spill).
+// SIMD (NV = 16): the waits of one are the others' work (20000 x 50 filtered, five / six / seven: 795 / 842 / 894 us, six and seven
+// spill; of an earlier state, four / five: 1111 / 960).
 template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64, NV == 16 ? 5 : 4) choose_kernel(Choice g) {
     extern __shared__ int s_tables[];                         // of up to MAX_LDS_FEATURES features: offsets, order
     __shared__ int s_start[5];
@@ -862,7 +864,7 @@ template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64
         const int K = __builtin_amdgcn_readfirstlane(order ? max(0, s_off[f + 1] - k0) : classes_of(g, f));
         if (++w == n) { w = 0; ++b; }
         // A lane a 64-byte piece of the row from the next block on: its lines are on their way while this one is worked on
-        // (20000 x 50 filtered 960 -> 890 us; to the end of a block as wide as this one 920; the next logits and uniforms kept
+        // (20000 x 50 filtered, then 960, 890 us; to the end of a block as wide as this one 920; the next logits and uniforms kept
         // in registers 1240, from 48 of them spilled)
         float touched = 0.f;
         auto ahead = [&] {
@@ -888,9 +890,9 @@ template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64
 
 // ------------------------------------------------------------------------------------------- very many classes, in chunks
 // Four launches over chunks of a block (top -> bins -> collect) and over blocks (finish).  Weights are integers, so that the
-// sums over chunks have no order.  64 x 131071 bfloat16 with top-p: 6.6 + 17.8 + 15.3 + 17.0 us; reading it once takes 3.6.  The
+// sums over chunks have no order.  64 x 131071 bfloat16 with top-p: 6.7 + 16.2 + 13.0 + 17.0 us; reading it once takes 3.6.  The
 // second is bound by its masses (8.4 million float64 exponentials), the others by the latency of a few dependent loads and
-// workgroup sums; so are all four of 1 x 262144 with top-k (3.0 + 7.6 + 6.3 + 9.9).  Between the launches, for every wide block
+// workgroup sums; so are all four of 1 x 262144 with top-k (3.0 + 7.6 + 6.4 + 10.0).  Between the launches, for every wide block
 // and in `ws`:
 constexpr int WT = 256, WIDE_BINS = 256, WIDE_LIST = 4096, WIDE_CHUNKS = 1024;
 struct Wide {
