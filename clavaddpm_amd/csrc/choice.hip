@@ -74,11 +74,25 @@ __device__ __forceinline__ double exp2_nonpos(double y) {
     constexpr Exp2Terms c;
     y = fmax(y, -1100.0);
     const double n = rint(y), r = y - n;
-    double p = c.t[11];
-    // (written out, since the terms belong in scalar registers: the compiler kept 22 vector registers of them and copied one for
-    // every step; 20000 x 50 filtered 884 -> 795 us together with lane moves that need no zero first)
-#pragma unroll
-    for (int k = 10; k >= 1; --k) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p) : "v"(p), "v"(r), "s"(c.t[k]));
+    // Written out, since the terms belong in scalar registers: the compiler kept 22 vector registers of them and copied one for
+    // every step (20000 x 50 filtered 884 -> 795 us together with lane moves that need no zero first).  The wait is for scalar
+    // registers that a vector instruction wrote just before (a v_readlane of spilled ones): two states, which the compiler does
+    // not count for written-out code.
+    double p;
+    asm("s_nop 1\n\t"
+        "v_fma_f64 %0, %1, %2, %3\n\t"
+        "v_fma_f64 %0, %0, %2, %4\n\t"
+        "v_fma_f64 %0, %0, %2, %5\n\t"
+        "v_fma_f64 %0, %0, %2, %6\n\t"
+        "v_fma_f64 %0, %0, %2, %7\n\t"
+        "v_fma_f64 %0, %0, %2, %8\n\t"
+        "v_fma_f64 %0, %0, %2, %9\n\t"
+        "v_fma_f64 %0, %0, %2, %10\n\t"
+        "v_fma_f64 %0, %0, %2, %11\n\t"
+        "v_fma_f64 %0, %0, %2, %12"
+        : "=&v"(p)
+        : "v"(c.t[11]), "v"(r), "s"(c.t[10]), "s"(c.t[9]), "s"(c.t[8]), "s"(c.t[7]), "s"(c.t[6]), "s"(c.t[5]), "s"(c.t[4]),
+          "s"(c.t[3]), "s"(c.t[2]), "s"(c.t[1]));
     return ldexp(fma(p, r, 1.0), (int)n);
 }
 // log(x) for x >= 1: the float32 logarithm and one Newton step on e^y = x (its square, 1e-14, is what stays)
