@@ -347,3 +347,21 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for k, t in got:
         assert torch.equal(t, want[k])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows, cols", [(1, 5), (1, 600), (2, 9), (3, 127), (37, 129), (300, 513), (64, 1999)])
+def test_rows_at_every_place_of_16_bytes(rows, cols, dtype):
+    """Rows that start anywhere in 16 bytes, of a tensor of their own (nothing before or behind) and inside a wider one."""
+    x = rand(rows, cols, cols).to(DEV)
+    ref = ops.mx4_pack(x.to(dtype).float())
+    for start in range(9):
+        for gap in (0, 1, 3, 8):
+            flat = torch.full((start + rows * (cols + gap) + 16,), math.nan, device=DEV, dtype=dtype)
+            view = flat[start:].as_strided((rows, cols), (cols + gap, 1), flat.storage_offset() + start)
+            view.copy_(x)
+            q = ops.mx4_pack(view)
+            assert torch.equal(q.codes, ref.codes) and torch.equal(q.scales, ref.scales), (start, gap)
+    own = x.to(dtype)
+    q = ops.mx4_pack(own)
+    assert torch.equal(q.codes, ref.codes) and torch.equal(q.scales, ref.scales)
