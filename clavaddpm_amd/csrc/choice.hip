@@ -558,13 +558,15 @@ __device__ __forceinline__ void choose_wave(const Choice& g, const Block& x, flo
             // few enough for a class a lane: everything else is done there
             int count = 0;
             float zl = -INFINITY;
-            // (its bin is at most `at`: all but -inf for the last one, whose product is inf or no number)
-            const float limit = at == 63 ? INFINITY : (float)(at + 1);
+            // Exactly the classes that were counted into bins up to `at`: where that is the last bin (which has those, too, whose
+            // product passes float32: the type's lowest value under an ordinary maximum) or the only one, all above -inf
+            const bool all = at == 63 || w.inv == 0.f;
+            const float limit = (float)(at + 1);
             lds_order();
 #pragma unroll 2
             for (int j = 0; j < w.n; ++j) {
                 const float z = zs[j * 64 + lane];
-                const bool is = (top - z) * w.inv < limit;
+                const bool is = all ? z > -INFINITY : (top - z) * w.inv < limit;
                 const u64 who = __ballot(is);
                 const int pos = count + (int)__popcll(who & ((1ull << lane) - 1));
                 if (is) s.place[pos] = (u64)__float_as_uint(z) << 32 | (unsigned)(j * 64 + lane);
@@ -572,8 +574,8 @@ __device__ __forceinline__ void choose_wave(const Choice& g, const Block& x, flo
             }
             lds_order();
             const u64 mine = s.place[lane];
-            if (lane < n) zl = __uint_as_float((unsigned)(mine >> 32));
-            choose_lanes<64, MODE>(g, x, zl, lane < n ? key_of(zl) : 0u, (int)(unsigned)mine, top, false, true, &chosen);
+            if (lane < count) zl = __uint_as_float((unsigned)(mine >> 32));
+            choose_lanes<64, MODE>(g, x, zl, lane < count ? key_of(zl) : 0u, (int)(unsigned)mine, top, false, true, &chosen);
             return;
         }
         edge = find_edge(w, (u64)bin, (double)x.top_k, s, in, one);
