@@ -281,23 +281,25 @@ __global__ void __launch_bounds__(WN * WM * 64) mx4_tile_kernel(Mx4Args g, int t
             }
         }
     };
-    // Stages s + 1 .. s + NS - 1 are on their way while stage s is multiplied; the counted wait says that stage s is there
+    // Stages s + 1 .. s + NS - 1 are on their way while stage s is multiplied; the counted wait says that stage s is there.  Behind
+    // the barrier other waves' copies (or strips) go to where this one has read: its reads have returned by then, wherever the
+    // compiler has put the products that use them.
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) copy(s, smem + s * STAGE);
     int cur = 0, nxt = (NS - 1) * STAGE;
     for (int s = 0; s < g.ks >> 1; ++s) {
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WAIT) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WAIT) : "memory");
         copy(s + NS - 1, smem + nxt);
         multiply(smem + cur, s, std::integral_constant<int, 4>{});
         nxt = cur;
         cur = cur + STAGE == NS * STAGE ? 0 : cur + STAGE;
     }
     if (!S16 && (g.ks & 1)) {
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WAIT) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WAIT) : "memory");
         multiply(smem + cur, stages - 1, std::integral_constant<int, 2>{});
     }
     // the last copies land, and nobody reads the stages any more: their LDS is free
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (OUT == OUT_MX4) {
 #pragma unroll
         for (int i = 0; i < TN; ++i) {
