@@ -426,7 +426,10 @@ template <int OUT> int launch_linear(const Mx4Args& g, hipStream_t st) {
     // 27.7 / 23.3 / 38.8, 4096 x 1024 x 1024 13.9 / 7.7 / 10.3, 1024 x 1024 x 1024 13.0 / 6.4 / 4.7, 256 x 4096 x 4096
     // 30.2 / 13.0 / 8.4).
     auto tiles = [&](int t) { return (long long)((g.M + t - 1) / t) * ((n_cols + t - 1) / t); };
-    if (g.M > 64) {
+    // The tiles copy scales by dwords.  Those that start between two (a view into a loaded file) are read by bytes, as those of few
+    // rows are: right for any number of rows, but 16 rows at a time.
+    const bool dwords = (((uintptr_t)g.xs | (uintptr_t)g.ws) & 3) == 0;
+    if (g.M > 64 && dwords) {
         if (tiles(256) >= 512) return launch_tile<256, 256, 2, 4, 2, OUT>(g, n_cols, st);
         if (tiles(128) >= 256) return launch_tile<128, 128, 2, 4, 2, OUT>(g, n_cols, st);
         return launch_tile<64, 64, 2, 2, 4, OUT>(g, n_cols, st);
@@ -471,7 +474,8 @@ int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_sc
     const bool x4 = x_dtype == CLAVA_DT_MX4, y4 = y_dtype == CLAVA_DT_MX4;
     CLAVA_CHECK_ARG(x && w_codes && w_scales && y && (!y4 || y_scales) && (x4 ? x_scales != nullptr : !packed_first(M, K) || workspace), "linear_mx4: null pointer");
     CLAVA_CHECK_ARG(y4 || ldy >= N || M == 1, "linear_mx4: leading dimension %lld below %d columns", ldy, N);
-    CLAVA_CHECK_ARG((((uintptr_t)(x4 ? x : packed_first(M, K) ? workspace : nullptr) | (uintptr_t)w_codes) & 15) == 0, "linear_mx4: codes and workspace start at 16 bytes");
+    CLAVA_CHECK_ARG((((uintptr_t)(x4 ? x : packed_first(M, K) ? workspace : nullptr) | (uintptr_t)w_codes | (uintptr_t)(y4 ? y : nullptr)) & 15) == 0,
+                    "linear_mx4: codes and workspace start at 16 bytes");
     CLAVA_CHECK_ARG(N <= 0x7fffff00 && K <= 0x7fffff00 && M <= 0x7fffff00, "linear_mx4: M %d, N %d, K %d", M, N, K);
     if (K > MOST_COLUMNS) {
         clava_set_error("linear_mx4: %d columns are more than one call takes (%d)", K, MOST_COLUMNS);

@@ -94,6 +94,7 @@ int clava_mx4_pack(const void* src, int dtype, long long ld, long long rows, int
     if (rows == 0) return CLAVA_OK;
     CLAVA_CHECK_ARG(src && codes && scales, "mx4_pack: null pointer");
     CLAVA_CHECK_ARG(dtype >= 0 && dtype <= CLAVA_DT_F16, "mx4_pack: dtype %d", dtype);
+    CLAVA_CHECK_ARG(((uintptr_t)codes & 3) == 0, "mx4_pack: codes start at 4 bytes");
     CLAVA_CHECK_ARG(ld >= cols || rows == 1, "mx4_pack: leading dimension %lld below %d columns", ld, cols);
     CLAVA_CHECK_ARG(cols <= 0x7fffff80, "mx4_pack: %d columns", cols);
     const hipStream_t st = (hipStream_t)stream;
@@ -122,6 +123,7 @@ int clava_mx4_unpack(const void* codes, const void* scales, long long rows, int 
     if (rows == 0) return CLAVA_OK;
     CLAVA_CHECK_ARG(dst && codes && scales, "mx4_unpack: null pointer");
     CLAVA_CHECK_ARG(dtype >= 0 && dtype <= CLAVA_DT_F16, "mx4_unpack: dtype %d", dtype);
+    CLAVA_CHECK_ARG(((uintptr_t)codes & 3) == 0, "mx4_unpack: codes start at 4 bytes");
     CLAVA_CHECK_ARG(ld >= cols || rows == 1, "mx4_unpack: leading dimension %lld below %d columns", ld, cols);
     CLAVA_CHECK_ARG(cols <= 0x7fffff80, "mx4_unpack: %d columns", cols);
     const hipStream_t st = (hipStream_t)stream;

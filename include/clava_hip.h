@@ -155,8 +155,9 @@ int clava_gemm_wgrad_f16x3_tn(const void* dy, long long pitch_dy, int shift_dy, 
  * clava_linear_mx4: y[M,N] = act( x[M,K] . w[N,K]^T + bias[N] ), products summed in float32; w as above, x as above (x_dtype
  *   CLAVA_DT_MX4: `x` its codes, x_scales) or a float matrix of row stride ldx, which is packed as clava_mx4_pack does, into
  *   `workspace` (clava_linear_mx4_workspace_bytes(M, K, x_dtype) bytes, 16-byte aligned; NULL where that is 0).  The result as `y` (y_dtype, row stride ldy) or,
- *   with y_dtype CLAVA_DT_MX4, packed again (`y` its codes, y_scales; for the next layer).  codes pointers are 16-byte
- *   aligned; K at most 2^25.  y may not overlap x.  dtype: CLAVA_DT_*; act: CLAVA_ACT_*_. */
+ *   with y_dtype CLAVA_DT_MX4, packed again (`y` its codes, y_scales; for the next layer).  K at most 2^25.  y may not overlap x.
+ * codes start at a multiple of 16 bytes (for pack and unpack 4 are enough); scales may start anywhere, but a product of more than
+ * 64 rows is slow with scales that do not start at a multiple of 4.  dtype: CLAVA_DT_*; act: CLAVA_ACT_*_. */
 int clava_mx4_pack(const void* src, int dtype, long long ld, long long rows, int cols, void* codes, void* scales, void* stream);
 int clava_mx4_unpack(const void* codes, const void* scales, long long rows, int cols, void* dst, int dtype, long long ld, void* stream);
 long long clava_linear_mx4_workspace_bytes(int M, int K, int x_dtype);

@@ -1,6 +1,10 @@
 """What the low-bit layers and the filtered draws check on the host, and what their sources have to hold (no GPU needed)."""
+import ctypes
 import os
 import re
+
+from clavaddpm_amd import ops
+from clavaddpm_amd._lib import lib
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "clavaddpm_amd", "csrc")
 
@@ -13,3 +17,20 @@ def test_a_waves_lds_reads_have_returned_before_it_passes_a_barrier_of_the_produ
     assert len(barriers) == 3
     for b in barriers:
         assert re.fullmatch(r"s_waitcnt vmcnt\((%0|0)\) lgkmcnt\(0\)\\n\\ts_barrier", b), b
+
+
+def c_refuses(name, types, *args):
+    rc = ops._function(name, types)(*args, None)
+    assert rc < 0
+    return lib().clava_last_error().decode()
+
+
+def test_codes_have_to_start_where_their_loads_and_stores_do():
+    p, off = ctypes.c_void_p(4096), ctypes.c_void_p(4096 + 2)
+    assert "codes" in c_refuses("clava_mx4_pack", "pillippp", p, 0, 40, 4, 40, off, p)
+    assert "codes" in c_refuses("clava_mx4_unpack", "pplipilp", off, p, 4, 40, p, 0, 40)
+    layer = [p, 3, 0, p, p, p, None, 0, p, 3, 0, p, 4, 8, 40, None]
+    for at in (0, 4, 8):                                         # x, w, y
+        args = list(layer)
+        args[at] = ctypes.c_void_p(4096 + 4)
+        assert "16 bytes" in c_refuses("clava_linear_mx4", "pilppppipilpiiipp", *args), at
