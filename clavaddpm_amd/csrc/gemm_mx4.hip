@@ -464,9 +464,9 @@ long long clava_linear_mx4_workspace_bytes(int M, int K, int x_dtype) {
     return M > 0 && K > 0 && packed_first(M, K) && x_dtype != CLAVA_DT_MX4 ? (long long)M * steps(K) * 68 : 0;
 }
 
-int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_scales, const void* w_codes, const void* w_scales,
-                     const float* bias, int act, void* y, int y_dtype, long long ldy, void* y_scales, int M, int N, int K,
-                     void* workspace, void* stream) {
+int clava_linear_mx4_sized(const void* x, int x_dtype, long long ldx, const void* x_scales, const void* w_codes, const void* w_scales,
+                           const float* bias, int act, void* y, int y_dtype, long long ldy, void* y_scales, int M, int N, int K,
+                           void* workspace, long long workspace_bytes, void* stream) {
     CLAVA_CHECK_ARG(M >= 0 && N > 0 && K > 0, "linear_mx4: M %d, N %d, K %d", M, N, K);
     CLAVA_CHECK_ARG(act >= CLAVA_ACT_NONE && act <= CLAVA_ACT_SILU, "linear_mx4: activation %d", act);
     CLAVA_CHECK_ARG(x_dtype >= 0 && x_dtype <= CLAVA_DT_MX4 && y_dtype >= 0 && y_dtype <= CLAVA_DT_MX4, "linear_mx4: dtypes %d, %d", x_dtype, y_dtype);
@@ -487,7 +487,9 @@ int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_sc
     g.xq = (const char*)x; g.xs = (const unsigned char*)x_scales;
     g.xt = x_dtype; g.K = K; g.ldx = ldx;
     CLAVA_CHECK_ARG(x4 || ldx >= K || M == 1, "linear_mx4: leading dimension %lld below %d columns", ldx, K);
-    if (!x4 && packed_first(M, K)) {
+    const long long need = clava_linear_mx4_workspace_bytes(M, K, x_dtype);
+    CLAVA_CHECK_ARG(workspace_bytes >= need, "linear_mx4: needs a workspace of %lld bytes, got %lld", need, workspace_bytes);
+    if (need) {
         g.xt = CLAVA_DT_MX4;
         g.xq = (const char*)workspace;
         g.xs = (const unsigned char*)workspace + (size_t)M * g.ks * 64;
@@ -506,6 +508,13 @@ int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_sc
     if (rc) return rc;
     CLAVA_CHECK_LAUNCH("linear_mx4");
     return CLAVA_OK;
+}
+
+int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_scales, const void* w_codes, const void* w_scales,
+                     const float* bias, int act, void* y, int y_dtype, long long ldy, void* y_scales, int M, int N, int K,
+                     void* workspace, void* stream) {
+    // (a workspace of a size that nobody gave is taken to have none)
+    return clava_linear_mx4_sized(x, x_dtype, ldx, x_scales, w_codes, w_scales, bias, act, y, y_dtype, ldy, y_scales, M, N, K, workspace, 0, stream);
 }
 
 }  // extern "C"

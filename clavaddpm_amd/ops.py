@@ -466,8 +466,13 @@ def _overlap(a, row_a, step_a, b, row_b, step_b, rows):
     return d < row_a or d + row_b > step_a
 
 
+@functools.lru_cache(maxsize=256)
+def _mx4_workspace(rows, cols, dt):
+    return _function("clava_linear_mx4_workspace_bytes", "iii", c_ll)(rows, cols, dt)
+
+
 def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
-    """act(x @ w.T + bias) over 4-bit operands (clava_linear_mx4): `w` an Mx4Tensor [N, K], `x` an Mx4Tensor [M, K] or a float
+    """act(x @ w.T + bias) over 4-bit operands (clava_linear_mx4_sized): `w` an Mx4Tensor [N, K], `x` an Mx4Tensor [M, K] or a float
     matrix, which is packed first.  The result is a float matrix of `out_dtype`, or whatever `out` is: a float matrix or an
     Mx4Tensor (the next layer's operand); it may not overlap x.  No gradient is defined."""
     if not isinstance(w, Mx4Tensor):
@@ -511,11 +516,14 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
             _refuse(f"linear_mx4: the result is [{M},{N}] on {dev} but out is [{rows},{cols}] on {out.device}")
         if M and _overlap(xp, *_span(x, K, ldx), yp, *_span(out, N, ldy), M):
             _refuse("linear_mx4: out overlaps x, which is read while out is written")
-    if x_dt != _MX4 and (M > 16 or K > 2048):
-        ws = torch.empty(M * 68 * ((K + 127) // 128), device=dev, dtype=torch.uint8)      # clava_linear_mx4_workspace_bytes
-    _launch(dev, "clava_linear_mx4", _function("clava_linear_mx4", "pilppppipilpiiipp"),
+    need = 0
+    if x_dt != _MX4:
+        need = _mx4_workspace(M, K, x_dt)
+        if need:
+            ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    _launch(dev, "clava_linear_mx4_sized", _function("clava_linear_mx4_sized", "pilppppipilpiiiplp"),
             xp, x_dt, ldx, xs, w.codes_ptr, w.scales_ptr, bp, code, yp, y_dt, ldy, ys, M, N, K,
-            None if ws is None else ws.data_ptr())
+            None if ws is None else ws.data_ptr(), need)
     return out
 
 

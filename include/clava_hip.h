@@ -152,9 +152,10 @@ int clava_gemm_wgrad_f16x3_tn(const void* dy, long long pitch_dy, int shift_dy, 
  * clava_mx4_pack: scale exponent e = floor(log2(max |v|)) - 2 (clamped to -127 .. 127), code = nearest E2M1 of v / 2^e, ties to
  *   even, saturating at 6; a block that holds a NaN or an infinity gets scale 255 and reads as NaN.  src has row stride ld.
  * clava_mx4_unpack: dst[r * ld + c] = value(code) * 2^(scale - 127), rounded to `dtype`.
- * clava_linear_mx4: y[M,N] = act( x[M,K] . w[N,K]^T + bias[N] ), products summed in float32; w as above, x as above (x_dtype
+ * clava_linear_mx4_sized: y[M,N] = act( x[M,K] . w[N,K]^T + bias[N] ), products summed in float32; w as above, x as above (x_dtype
  *   CLAVA_DT_MX4: `x` its codes, x_scales) or a float matrix of row stride ldx, which is packed as clava_mx4_pack does, into
- *   `workspace` (clava_linear_mx4_workspace_bytes(M, K, x_dtype) bytes, 16-byte aligned; NULL where that is 0).  The result as `y` (y_dtype, row stride ldy) or,
+ *   `workspace` (16-byte aligned, of workspace_bytes >= clava_linear_mx4_workspace_bytes(M, K, x_dtype); NULL where that is 0).
+ *   clava_linear_mx4, without workspace_bytes, takes calls that need no workspace.  The result as `y` (y_dtype, row stride ldy) or,
  *   with y_dtype CLAVA_DT_MX4, packed again (`y` its codes, y_scales; for the next layer).  K at most 2^25.  y may not overlap x.
  * codes start at a multiple of 16 bytes (for pack and unpack 4 are enough); scales may start anywhere, but a product of more than
  * 64 rows is slow with scales that do not start at a multiple of 4.  dtype: CLAVA_DT_*; act: CLAVA_ACT_*_. */
@@ -164,6 +165,9 @@ long long clava_linear_mx4_workspace_bytes(int M, int K, int x_dtype);
 int clava_linear_mx4(const void* x, int x_dtype, long long ldx, const void* x_scales, const void* w_codes, const void* w_scales,
                      const float* bias, int act, void* y, int y_dtype, long long ldy, void* y_scales, int M, int N, int K,
                      void* workspace, void* stream);
+int clava_linear_mx4_sized(const void* x, int x_dtype, long long ldx, const void* x_scales, const void* w_codes, const void* w_scales,
+                           const float* bias, int act, void* y, int y_dtype, long long ldy, void* y_scales, int M, int N, int K,
+                           void* workspace, long long workspace_bytes, void* stream);
 
 /* ---- schedule tables ---------------------------------------------------------------------------------------
  * Device-resident tables of length T, built by the host exactly as GaussianMultinomialDiffusion.__init__ builds

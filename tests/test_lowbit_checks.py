@@ -34,3 +34,18 @@ def test_codes_have_to_start_where_their_loads_and_stores_do():
         args = list(layer)
         args[at] = ctypes.c_void_p(4096 + 4)
         assert "16 bytes" in c_refuses("clava_linear_mx4", "pilppppipilpiiipp", *args), at
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    """Float rows are packed into the workspace: 17 rows of 40 columns need 17 * 68 bytes."""
+    p = ctypes.c_void_p(4096)
+    need = ops._mx4_workspace(17, 40, 0)
+    assert need == 17 * 68
+    args = [p, 0, 40, None, p, p, None, 0, p, 0, 8, None, 17, 8, 40, p]
+    for size in (0, need - 1, -1):
+        said = c_refuses("clava_linear_mx4_sized", "pilppppipilpiiiplp", *args, size)
+        assert f"{need} bytes" in said and str(size) in said
+    assert f"{need} bytes" in c_refuses("clava_linear_mx4", "pilppppipilpiiipp", *args)      # of a size that nobody gave
+    small = list(args)
+    small[12], small[15] = 0, None                               # no rows: nothing to do
+    assert ops._function("clava_linear_mx4_sized", "pilppppipilpiiiplp")(*small, 0, None) == 0
