@@ -432,28 +432,28 @@ def mx4_pack(x, out=None):
         out = mx4_empty(rows, cols, x.device)
     elif (out.rows, out.cols) != (rows, cols) or out.device != x.device:
         _refuse(f"mx4_pack: x is [{rows},{cols}] on {x.device} but out is [{out.rows},{out.cols}] on {out.device}")
+    elif rows:
+        _not_over("mx4_pack", _parts(out, rows, cols, 0), x=_parts(x, rows, cols, ld))
     _launch(out.device, "clava_mx4_pack", _function("clava_mx4_pack", "pillippp"),
             x.data_ptr(), dt, ld, rows, cols, out.codes_ptr, out.scales_ptr)
     return out
 
 
 def mx4_unpack(q, dtype=torch.float32, out=None):
-    """The values of an Mx4Tensor as float32, bfloat16 or float16 (clava_mx4_unpack)."""
-    if out is None:
+    """The values of an Mx4Tensor as float32, bfloat16 or float16 (clava_mx4_unpack); `out` may not overlap it."""
+    own = out is None
+    if own:
         if dtype not in _DT:
             _refuse(f"mx4_unpack: expected float32, bfloat16 or float16, got {dtype}")
         out = torch.empty((q.rows, q.cols), device=q.device, dtype=dtype)
     rows, cols, ld = _matrix(out, "mx4_unpack: out")
     if (rows, cols) != (q.rows, q.cols) or out.device != q.device:
         _refuse(f"mx4_unpack: q is [{q.rows},{q.cols}] on {q.device} but out is [{rows},{cols}] on {out.device}")
+    if rows and not own:
+        _not_over("mx4_unpack", _parts(out, rows, cols, ld), q=_parts(q, rows, cols, 0))
     _launch(q.device, "clava_mx4_unpack", _function("clava_mx4_unpack", "pplipilp"),
             q.codes_ptr, q.scales_ptr, rows, cols, out.data_ptr(), _dt(out, "mx4_unpack: out"), ld)
     return out
-
-
-def _span(t, cols, ld):
-    """(bytes of a row, of its stride)"""
-    return (64 * ((cols + 127) // 128),) * 2 if isinstance(t, Mx4Tensor) else (cols * t.element_size(), ld * t.element_size())
 
 
 def _overlap(a, row_a, step_a, b, row_b, step_b, rows):
@@ -466,6 +466,43 @@ def _overlap(a, row_a, step_a, b, row_b, step_b, rows):
     return d < row_a or d + row_b > step_a
 
 
+def _parts(t, rows, cols, ld):
+    """The memory of an operand or result: (start, bytes of a row, of its stride, rows); codes and scales are one row each."""
+    if isinstance(t, Mx4Tensor):
+        steps = rows * ((cols + 127) // 128)
+        return (t.codes_ptr, 64 * steps, 64 * steps, 1), (t.scales_ptr, 4 * steps, 4 * steps, 1)
+    size = t.element_size()
+    return ((t.data_ptr(), cols * size, ld * size, rows),)
+
+
+def _spread(t):
+    """A tensor's memory as one part, with what lies between its elements."""
+    size = t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    return ((t.data_ptr(), size, size, 1),)
+
+
+def _share(p, q):
+    """Whether two such parts have a byte in common (of two matrices with strides that differ: whether they may)."""
+    (a, row_a, step_a, rows_a), (b, row_b, step_b, rows_b) = p, q
+    if rows_a == 1 and rows_b == 1 or rows_a == rows_b:
+        return _overlap(a, row_a, step_a, b, row_b, step_b, rows_a)
+    if rows_a == 1:
+        a, row_a, step_a, rows_a, b, row_b, rows_b = b, row_b, step_b, rows_b, a, row_a, rows_a
+    if rows_b > 1:
+        return a < b + (rows_b - 1) * step_b + row_b and b < a + (rows_a - 1) * step_a + row_a
+    i = max(0, (b - a - row_a) // step_a + 1)                    # the first row that ends behind b
+    return i < rows_a and a + i * step_a < b + row_b
+
+
+def _not_over(name, out, **inputs):
+    """Refuse a result that shares memory with what is read while it is written; all are tuples of parts."""
+    low, high = min(p[0] for p in out), max(a + (n - 1) * step + row for a, row, step, n in out)
+    for what, parts in inputs.items():
+        for p in parts:
+            if p[0] < high and low < p[0] + (p[3] - 1) * p[2] + p[1] and any(_share(p, q) for q in out):
+                _refuse(f"{name}: out overlaps {what}, which is read while out is written")
+
+
 @functools.lru_cache(maxsize=256)
 def _mx4_workspace(rows, cols, dt):
     return _function("clava_linear_mx4_workspace_bytes", "iii", c_ll)(rows, cols, dt)
@@ -474,7 +511,7 @@ def _mx4_workspace(rows, cols, dt):
 def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
     """act(x @ w.T + bias) over 4-bit operands (clava_linear_mx4_sized): `w` an Mx4Tensor [N, K], `x` an Mx4Tensor [M, K] or a float
     matrix, which is packed first.  The result is a float matrix of `out_dtype`, or whatever `out` is: a float matrix or an
-    Mx4Tensor (the next layer's operand); it may not overlap x.  No gradient is defined."""
+    Mx4Tensor (the next layer's operand); it may not overlap x, w or bias.  No gradient is defined."""
     if not isinstance(w, Mx4Tensor):
         _refuse("linear_mx4: w must be an Mx4Tensor")
     code = _ACT.get(act)
@@ -514,8 +551,9 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
             y_dt, yp, ys = _dt(out, "linear_mx4: out"), out.data_ptr(), None
         if (rows, cols) != (M, N) or out.device != dev:
             _refuse(f"linear_mx4: the result is [{M},{N}] on {dev} but out is [{rows},{cols}] on {out.device}")
-        if M and _overlap(xp, *_span(x, K, ldx), yp, *_span(out, N, ldy), M):
-            _refuse("linear_mx4: out overlaps x, which is read while out is written")
+        if M:
+            _not_over("linear_mx4", _parts(out, M, N, ldy), x=_parts(x, M, K, ldx), w=_parts(w, N, K, 0),
+                      bias=((bp, 4 * N, 4 * N, 1),) if bp else ())
     need = 0
     if x_dt != _MX4:
         need = _mx4_workspace(M, K, x_dt)
@@ -606,6 +644,11 @@ def sample_categories(logits, uniforms=None, offsets=None, max_classes=None, *, 
         out = torch.empty((B, m), device=dev, dtype=torch.int32)
     elif out.dtype is not torch.int32 or out.shape != (B, m) or not out.is_contiguous() or out.device != dev:
         _refuse(f"sample_categories: out must be contiguous int32 [{B},{m}] on {dev}")
+    elif B:
+        row = 4 * m
+        whole = {n: _spread(v) for n, v in zip(_CHOICE_RANGE, (temperature, top_p, min_p, top_k)) if isinstance(v, torch.Tensor) and v.numel()}
+        _not_over("sample_categories", ((out.data_ptr(), B * row, B * row, 1),), logits=_parts(logits, B, sumk, ld) if sumk else (),
+                  offsets=((op, row + 4, row + 4, 1),) if op else (), uniforms=_parts(uniforms, B, m, ld_u) if up else (), **whole)
     values = temperature, top_p, min_p, top_k
     c = _choice_numbers(*values) if _NUMBERS.issuperset(map(type, values)) else _choice_args(dev, B, m, zip(_CHOICE_RANGE, values))
     lp = torch.empty((B, m), device=dev, dtype=torch.float32) if log_prob else None

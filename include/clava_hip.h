@@ -156,7 +156,7 @@ int clava_gemm_wgrad_f16x3_tn(const void* dy, long long pitch_dy, int shift_dy, 
  *   CLAVA_DT_MX4: `x` its codes, x_scales) or a float matrix of row stride ldx, which is packed as clava_mx4_pack does, into
  *   `workspace` (16-byte aligned, of workspace_bytes >= clava_linear_mx4_workspace_bytes(M, K, x_dtype); NULL where that is 0).
  *   clava_linear_mx4, without workspace_bytes, takes calls that need no workspace.  The result as `y` (y_dtype, row stride ldy) or,
- *   with y_dtype CLAVA_DT_MX4, packed again (`y` its codes, y_scales; for the next layer).  K at most 2^25.  y may not overlap x.
+ *   with y_dtype CLAVA_DT_MX4, packed again (`y` its codes, y_scales; for the next layer).  K at most 2^25.  y may not overlap x, w or bias.
  * codes start at a multiple of 16 bytes (for pack and unpack 4 are enough); scales may start anywhere, but a product of more than
  * 64 rows is slow with scales that do not start at a multiple of 4.  dtype: CLAVA_DT_*; act: CLAVA_ACT_*_. */
 int clava_mx4_pack(const void* src, int dtype, long long ld, long long rows, int cols, void* codes, void* scales, void* stream);
@@ -248,7 +248,7 @@ int clava_categorical_sampler_set(int mode);
  * temperature 0 takes the first of the order.  A class with z = -inf is never drawn; where some z are +inf, those share the
  * mass equally.  idx[b * m + f] = -1 (log_prob NaN) for a feature without classes, without a z above -inf, or with a NaN in
  * its logits, its u or a parameter, or a negative temperature.  log_prob (optional) [B, m]: log of the drawn class's share of
- * the kept mass.  Sums and comparisons are float64 and have a fixed order.
+ * the kept mass.  idx and log_prob may not overlap what is read.  Sums and comparisons are float64 and have a fixed order.
  * Each parameter is a number for all blocks, or, where its pointer is not NULL, element [b * rs + f * fs] of a device array.
  * uniforms [b * ld_u + f] in [0, 1), or NULL for the counter-based generator keyed by (seed, row_offset + b, f, step_index).
  * max_k: the largest number of classes of one feature (it picks the kernels and the workspace; any value is safe, a feature of

@@ -6,6 +6,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from clavaddpm_amd import ops
+from clavaddpm_amd._lib import ClavaHipError
 from test_gpu_mx4 import product_case, tolerance
 
 DEV = "cuda"
@@ -40,3 +41,34 @@ def test_scales_at_every_place_of_16_bytes(M, N, K):
         assert torch.equal(out.codes, again.codes) and torch.equal(out.scales, again.scales), start
         few = ops.linear_mx4(ops.mx4_pack(x[:9].to(DEV)), ws, b)
         assert torch.equal(few, ops.linear_mx4(ops.mx4_pack(x[:9].to(DEV)), wq, b)), start
+
+
+def test_results_over_weights_bias_and_scales():
+    x, w, bias = torch.randn(128, 128, device=DEV), ops.mx4_pack(torch.randn(128, 128, device=DEV)), torch.randn(128, device=DEV)
+    q = ops.mx4_pack(x)
+    both = torch.zeros(128, 256, device=DEV)
+    both[7, 200:] = 1.0
+    square = torch.randn(128, 128, device=DEV)
+    want = ops.linear_mx4(x, w, both[7, 128:].contiguous())
+    for f in (lambda: ops.linear_mx4(x, w, out=w), lambda: ops.linear_mx4(q, w, bias, out=w), lambda: ops.linear_mx4(x, w, square[3], out=square),
+              lambda: ops.linear_mx4(q, w, out=ops.Mx4Tensor(ops.mx4_empty(128, 128, DEV).codes, q.scales, 128)),
+              lambda: ops.linear_mx4(x, w, both[7, 100:228], out=both[:, :128]),
+              lambda: ops.mx4_pack(square, out=ops.Mx4Tensor(square.view(torch.uint8).view(-1)[:8192].view(128, 64), w.scales, 128)),
+              lambda: ops.mx4_unpack(ops.Mx4Tensor(square.view(torch.uint8).view(-1)[:8192].view(128, 64), w.scales, 128), out=square)):
+        with pytest.raises(ClavaHipError, match="overlaps"):
+            f()
+    # beside each other in one buffer
+    ops.linear_mx4(x, w, both[7, 128:], out=both[:, :128])
+    assert torch.equal(both[:, :128], want)
+
+
+def test_draws_over_what_they_read():
+    z, u = torch.randn(8, 8, device=DEV), torch.rand(8, 4, device=DEV)
+    off = torch.arange(0, 10, 2, device=DEV, dtype=torch.int32)
+    k = torch.full((8, 4), 2, device=DEV, dtype=torch.int32)
+    for f in (lambda: ops.sample_categories(z, u, off, out=z.view(torch.int32).view(-1)[16:48].view(8, 4)), lambda: ops.sample_categories(z, u, off, out=u.view(torch.int32)),
+              lambda: ops.sample_categories(z[:1], u[:1], off, out=off[1:].view(1, 4)), lambda: ops.sample_categories(z, u, off, top_k=k, out=k)):
+        with pytest.raises(ClavaHipError, match="overlaps"):
+            f()
+    out = torch.empty(8, 4, device=DEV, dtype=torch.int32)
+    assert torch.equal(ops.sample_categories(z, u, off, top_k=k, out=out), ops.sample_categories(z, u, off, top_k=2))

@@ -3,8 +3,11 @@ import ctypes
 import os
 import re
 
+import pytest
+import torch
+
 from clavaddpm_amd import ops
-from clavaddpm_amd._lib import lib
+from clavaddpm_amd._lib import ClavaHipError, lib
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "clavaddpm_amd", "csrc")
 
@@ -49,3 +52,42 @@ def test_a_workspace_that_is_too_small_is_refused():
     small = list(args)
     small[12], small[15] = 0, None                               # no rows: nothing to do
     assert ops._function("clava_linear_mx4_sized", "pilppppipilpiiiplp")(*small, 0, None) == 0
+
+
+def some_mx4(codes, scales, rows, cols):
+    """An Mx4Tensor at made-up addresses: calls on it are refused before anything reads them."""
+    q = ops.Mx4Tensor.__new__(ops.Mx4Tensor)
+    q.codes_ptr, q.scales_ptr, q.rows, q.cols, q.device = codes, scales, rows, cols, torch.device("cpu")
+    return q
+
+
+def test_a_result_over_anything_that_is_read_is_refused():
+    """64 x 128 matrices: codes of 4096 bytes, scales of 256."""
+    x, w = some_mx4(0x10000, 0x20000, 64, 128), some_mx4(0x30000, 0x40000, 64, 128)
+    for codes, scales, word in ((0x30000, 0x50000, "w"), (0x31000 - 16, 0x50000, "w"), (0x40000, 0x50000, "w"), (0x50000, 0x40000 + 255, "w"),
+                                (0x50000, 0x20000, "x"), (0x10000 - 4080, 0x50000, "x"), (0x20000, 0x30000, "x"), (0x50000, 0x30000 - 255, "w")):
+        with pytest.raises(ClavaHipError, match=f"overlaps {word},"):
+            ops.linear_mx4(x, w, out=some_mx4(codes, scales, 64, 64))
+    far = ops._parts(some_mx4(0x50000, 0x51000, 64, 128), 64, 128, 0)
+    ops._not_over("", far, x=ops._parts(x, 64, 128, 0), w=ops._parts(w, 64, 128, 0), bias=())
+    ops._not_over("", far, bias=((0x50000 - 512, 512, 512, 1),), b2=((0x51100, 512, 512, 1),))
+    for bias in ((0x50000 - 511, 512, 512, 1), (0x51100 - 1, 512, 512, 1), (0x50100, 4, 4, 1), (0x40000, 0x20000, 0x20000, 1)):
+        with pytest.raises(ClavaHipError, match="overlaps bias"):
+            ops._not_over("", far, bias=(bias,))
+
+
+def test_shared_bytes_of_rows_and_of_one_piece():
+    """Against the bytes themselves: rows of 6 bytes every 10 and pieces of every size and place, and other rows."""
+    def own(start, row, step, rows):
+        return {start + i * step + k for i in range(rows) for k in range(row)}
+    rows = (100, 6, 10, 4)
+    for start in range(90, 150):
+        for size in range(1, 25):
+            piece = (start, size, size, 1)
+            want = bool(own(*rows) & own(*piece))
+            assert ops._share(rows, piece) == want and ops._share(piece, rows) == want, piece
+        other = (start, 3, 10, 4)
+        assert ops._share(rows, other) == bool(own(*rows) & own(*other)) or start >= 130 or start < 73, start
+        assert ops._share(rows, (start, 3, 7, 2)) >= bool(own(*rows) & own(start, 3, 7, 2)), start
+    t = torch.zeros(5, 4)[:, 1:3]
+    assert ops._spread(t) == ((t.data_ptr(), 72, 72, 1),) and ops._spread(torch.zeros(1).expand(9)) [0][1] == 4
