@@ -9,6 +9,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import c_float, c_int, check, lib, ptr, require_cuda, stream_ptr
@@ -346,6 +347,14 @@ def _matrix(t, name):
     return rows, cols, ld
 
 
+def _no_gradient(message, *tensors):
+    """Refuse tensors that a derivative is asked of: recorded for backward, or duals with a tangent."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _refuse(message + ": call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _refuse(message + " and no forward derivative: give it the primal of a dual tensor")
+
+
 def _same_device(dev, **tensors):
     for name, t in tensors.items():
         if t is not None and t.device != dev:
@@ -426,8 +435,7 @@ def mx4_pack(x, out=None):
     that holds a NaN or an infinity reads as NaN.  No gradient is defined."""
     rows, cols, ld = _matrix(x, "mx4_pack: x")
     dt = _dt(x, "mx4_pack: x")
-    if x.requires_grad and torch.is_grad_enabled():
-        _refuse("mx4_pack has no backward: call it under torch.no_grad() or detach its input")
+    _no_gradient("mx4_pack has no backward", x)
     if out is None:
         out = mx4_empty(rows, cols, x.device)
     elif (out.rows, out.cols) != (rows, cols) or out.device != x.device:
@@ -523,8 +531,7 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
     else:
         M, K, ldx = _matrix(x, "linear_mx4: x")
         x_dt, xp, xs = _dt(x, "linear_mx4: x"), x.data_ptr(), None
-        if x.requires_grad and torch.is_grad_enabled():
-            _refuse("linear_mx4 has no backward: call it under torch.no_grad() or detach its inputs")
+        _no_gradient("linear_mx4 has no backward", x)
     if w.cols != K:
         _refuse(f"linear_mx4: x is [{M},{K}] but w is [{N},{w.cols}]")
     if N == 0:
@@ -535,8 +542,7 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
     if bias is not None:
         if bias.dtype is not torch.float32 or bias.shape != (N,) or not bias.is_contiguous() or bias.device != dev:
             _refuse(f"linear_mx4: bias must be contiguous float32 [{N}] on {dev}")
-        if bias.requires_grad and torch.is_grad_enabled():
-            _refuse("linear_mx4 has no backward: call it under torch.no_grad() or detach its inputs")
+        _no_gradient("linear_mx4 has no backward", bias)
         bp = bias.data_ptr()
     if out is None:
         if out_dtype not in _DT:
@@ -620,8 +626,8 @@ def sample_categories(logits, uniforms=None, offsets=None, max_classes=None, *, 
     and NaN.  A captured call repeats its own draws: give it `uniforms` that the program refills."""
     B, sumk, ld = _matrix(logits, "sample_categories: logits")
     dt = _dt(logits, "sample_categories: logits")
-    if log_prob and logits.requires_grad and torch.is_grad_enabled():
-        _refuse("sample_categories: log_prob has no backward: call it under torch.no_grad() or detach the logits")
+    if log_prob:
+        _no_gradient("sample_categories: log_prob has no backward", logits, temperature if isinstance(temperature, torch.Tensor) else None)
     dev = logits.device
     m, op = 1, None
     if offsets is not None:

@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +73,19 @@ def test_draws_over_what_they_read():
             f()
     out = torch.empty(8, 4, device=DEV, dtype=torch.int32)
     assert torch.equal(ops.sample_categories(z, u, off, top_k=k, out=out), ops.sample_categories(z, u, off, top_k=2))
+
+
+def test_tangents_are_refused_not_lost():
+    x, w = torch.randn(4, 40, device=DEV), ops.mx4_pack(torch.randn(8, 40, device=DEV))
+    t = torch.ones(4, 1, device=DEV)
+    want = ops.linear_mx4(x, w), ops.sample_categories(x, seed=3)
+    with forward_ad.dual_level():
+        dx, db, dt = (forward_ad.make_dual(v, torch.ones_like(v)) for v in (x, torch.zeros(8, device=DEV), t))
+        for f in (lambda: ops.mx4_pack(dx), lambda: ops.linear_mx4(dx, w), lambda: ops.linear_mx4(x, w, db),
+                  lambda: ops.sample_categories(dx, log_prob=True), lambda: ops.sample_categories(x, temperature=dt, log_prob=True)):
+            with pytest.raises(ClavaHipError, match="forward"):
+                f()
+        # whole numbers have no derivative, and inputs without a tangent are as ever
+        assert torch.equal(ops.sample_categories(dx, temperature=dt, seed=3), want[1]) and torch.equal(ops.linear_mx4(x, w), want[0])
+    with pytest.raises(ClavaHipError, match="backward"):
+        ops.sample_categories(x, temperature=t.clone().requires_grad_(), log_prob=True)

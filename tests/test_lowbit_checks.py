@@ -5,6 +5,7 @@ import re
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from clavaddpm_amd import ops
 from clavaddpm_amd._lib import ClavaHipError, lib
@@ -91,3 +92,22 @@ def test_shared_bytes_of_rows_and_of_one_piece():
         assert ops._share(rows, (start, 3, 7, 2)) >= bool(own(*rows) & own(start, 3, 7, 2)), start
     t = torch.zeros(5, 4)[:, 1:3]
     assert ops._spread(t) == ((t.data_ptr(), 72, 72, 1),) and ops._spread(torch.zeros(1).expand(9)) [0][1] == 4
+
+
+def test_a_derivative_that_is_asked_for_is_refused():
+    x = torch.ones(3)
+    ops._no_gradient("f has no backward", x, None)
+    with pytest.raises(ClavaHipError, match="f has no backward: call"):
+        ops._no_gradient("f has no backward", None, x.clone().requires_grad_())
+    with torch.no_grad():
+        ops._no_gradient("f has no backward", x.clone().requires_grad_())
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        ops._no_gradient("f has no backward", x, None)
+        ops._no_gradient("f has no backward", forward_ad.unpack_dual(dual).primal)
+        for grad in (True, False):                               # (no_grad does not stop tangents)
+            with torch.set_grad_enabled(grad), pytest.raises(ClavaHipError, match="no forward derivative"):
+                ops._no_gradient("f has no backward", x, dual)
+        w = some_mx4(0x30000, 0x40000, 3, 3)
+        with pytest.raises(ClavaHipError, match="no forward derivative"):
+            ops.linear_mx4(some_mx4(0x10000, 0x20000, 4, 3), w, dual)
