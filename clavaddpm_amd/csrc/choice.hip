@@ -942,26 +942,29 @@ __device__ __forceinline__ WideWs wide_ws(const Wide& w, long long block) {
     s.any = (unsigned*)p;
     return s;
 }
-// The n-th wide feature, or -1.  Every thread of the workgroup calls it.
-__device__ __forceinline__ int wide_feature(const Choice& g, int n, int* s_n) {
+// The n-th wide feature, or -1 (`s_n[0]`; ALL: and how many there are, `s_n[1]`).  Every thread of the workgroup calls it.
+template <bool ALL = false> __device__ __forceinline__ int wide_feature(const Choice& g, int n, int* s_n) {
     if (g.m == 1) return n == 0 && classes_of(g, 0) > g.wide_from ? 0 : -1;
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
-        int found = -1;
-        for (int f0 = 0; f0 < g.m && found < 0; f0 += 64) {
+        int found = -1, before = 0;
+        for (int f0 = 0; f0 < g.m && (ALL || found < 0); f0 += 64) {
             const int K = classes_of(g, min(f0 + lane, g.m - 1));
             u64 who = __ballot(f0 + lane < g.m && K > g.wide_from && K <= g.wide_to);
             const int c = (int)__popcll(who);
-            if (n < c) {
-                for (int k = 0; k < n; ++k) who &= who - 1;
+            if (found < 0 && n - before < c) {
+                for (int k = before; k < n; ++k) who &= who - 1;
                 found = f0 + (int)__builtin_ctzll(who);
             }
-            n -= c;
+            before += c;
         }
-        if (lane == 0) *s_n = found;
+        if (lane == 0) {
+            s_n[0] = found;
+            if (ALL) s_n[1] = before;
+        }
     }
     __syncthreads();
-    return *s_n;
+    return s_n[0];
 }
 struct WideBlock {
     Block x;
@@ -972,9 +975,9 @@ struct WideBlock {
     double scale;
     float inv;
 };
-__device__ __forceinline__ bool wide_block(const Choice& g, const Wide& w, long long block, WideBlock& o, int* s_n) {
+template <bool ALL = false> __device__ __forceinline__ bool wide_block(const Choice& g, const Wide& w, long long block, WideBlock& o, int* s_n) {
     const int b = (int)(block / w.per_row);
-    const int f = wide_feature(g, (int)(block - (long long)b * w.per_row), s_n);
+    const int f = wide_feature<ALL>(g, (int)(block - (long long)b * w.per_row), s_n);
     if (f < 0) return false;
     o.x = block_of<TENSORS>(g, b, f, first_of(g, f), classes_of(g, f));
     o.s = wide_ws(w, block);
@@ -1085,11 +1088,21 @@ __device__ __forceinline__ void wide_look(WideBlock& o, const WideHead& h) {
 }
 
 template <int DT> __global__ void __launch_bounds__(WT) wide_top_kernel(Choice g, Wide w) {
-    __shared__ int s_n;
+    __shared__ int s_n[2];
     __shared__ TeamLds s_t;
     WideBlock o;
-    if (!wide_block(g, w, blockIdx.y, o, &s_n)) return;
+    if (!wide_block<true>(g, w, blockIdx.y, o, s_n)) return;
     const int c = blockIdx.x, t = threadIdx.x;
+    // Features that overlap (offsets that fall in between) can be more wide ones than a row has room for side by side: nobody
+    // draws those that are left, and the last one's first workgroup says so
+    if (c == 0 && g.m > w.per_row && (int)(blockIdx.y % (unsigned)w.per_row) == w.per_row - 1) {
+        const int wide = s_n[1];
+        for (int n = w.per_row; n < wide; ++n) {
+            __syncthreads();
+            const int f = wide_feature(g, n, s_n);
+            if (t == 0) give(g, o.x.b, f, -1, no_number());
+        }
+    }
     if (c == 0 && (w.k || w.p)) {
         if (t == 0) *o.s.listed = 0;
         o.s.mass[t] = 0;

@@ -239,7 +239,10 @@ int clava_multinomial_step_counter_f32(const clava_schedule* sched, int mode, in
 int clava_categorical_sampler_set(int mode);
 
 /* One class per (row, feature) block from its logits, filtered (no counterpart in the reference, whose draws are unfiltered).
- * Feature f of row b owns logits[b * ld + offsets[f] .. offsets[f+1]) (m features; offsets == NULL: one feature of sumK classes).
+ * Feature f of row b owns logits[b * ld + offsets[f] .. offsets[f+1]) (m features; offsets == NULL: one feature of sumK classes;
+ * offsets outside of 0 .. sumK count as their nearest bound, a feature whose end is not behind its start has no classes).
+ * Offsets are meant to rise.  Where they do not, so that features overlap, no more than sumK / 2049 features of more than 2048
+ * classes (and at most max_k) are drawn, and the others get -1.
  * With a_i = exp((z_i - max z) / temperature) and the classes ordered by falling z (equal ones by rising index):
  *   top_k:  the first top_k of the order stay (<= 0 or >= the feature's classes: all);
  *   top_p:  of those, the ones before which less than top_p of their mass lies (>= 1: all; the first always stays);

@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 
 from clavaddpm_amd import ops
 from clavaddpm_amd._lib import ClavaHipError
-from test_gpu_choice import check, uniforms
+from test_gpu_choice import check, choose, uniforms
 
 DEV = "cuda"
 
@@ -56,3 +56,23 @@ def test_only_lowest_values_and_minus_infinities(K):
         for dtype in (torch.float32, torch.bfloat16):
             check(z if dtype is torch.float32 else z.clamp(torch.finfo(dtype).min, torch.finfo(dtype).max).where(z.isfinite(), z).to(dtype),
                   uniforms(5, 1, K), [K], **p)
+
+
+@pytest.mark.parametrize("off", [[0, 5000, 0, 5000, 0, 5000, 100, 4000], [0, 2100, 0, 2200, 3, 2300, 9, 60, 0, 2049], [4999, 5000, 0, 5000, 0, 50, 0, 4500, 1, 2800, 2, 4700]])
+@pytest.mark.parametrize("p", [{}, {"top_k": 30, "top_p": 0.9}, {"top_k": 1500}])
+def test_features_that_overlap_are_drawn_or_marked(off, p):
+    """More wide features than a row of that many classes has side by side: nothing is left as it was.  Those there is room for
+    have their class, as all others do, and the rest -1."""
+    m, B = len(off) - 1, 5
+    z = 2 * torch.randn((B, max(off)), generator=torch.Generator().manual_seed(m))
+    u = uniforms(B, m, m)
+    out = torch.full((B, m), 777777, device=DEV, dtype=torch.int32)
+    _, lp = ops.sample_categories(z.to(DEV), u.to(DEV), torch.tensor(off, device=DEV, dtype=torch.int32), out=out, log_prob=True, **p)
+    full = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0, **p}
+    wide = [f for f in range(m) if off[f + 1] - off[f] > 2048]
+    left = wide[max(off) // 2049:]
+    assert left
+    want = [[-1 if f in left else choose(z[b, off[f]:max(off[f], off[f + 1])].double().numpy(), float(u[b, f]), **full)[0] for f in range(m)]
+            for b in range(B)]
+    assert out.cpu().tolist() == want
+    assert torch.equal(lp.isnan(), out < 0)
