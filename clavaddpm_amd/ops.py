@@ -600,7 +600,7 @@ def _choice_args(dev, rows, features, values):
             setattr(c, name + "_fs", fs)
             continue
         low, high = _CHOICE_RANGE[name]
-        if not low <= v <= high or name == "top_k" and v != int(v):
+        if not low <= v <= high or name == "top_k" and v != int(v) or isinstance(v, int) and v > 2 ** 1023:
             _refuse(f"sample_categories: {name} {v}, expected {'a whole number' if name == 'top_k' else f'in [{low}, {high}]'}")
         setattr(c, name, max(-1, min(int(v), 2 ** 31 - 1)) if name == "top_k" else v)
     return c

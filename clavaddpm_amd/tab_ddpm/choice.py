@@ -4,6 +4,7 @@ The reference draws from the plain posterior (`log_sample_categorical`, `tab_ddp
 a `CategoryChoice` narrows the draw of the chain's last step, or of a single `p_sample_index`, to the likelier classes.
 """
 import math
+import sys
 
 import torch
 
@@ -12,11 +13,12 @@ _FIELDS = ("temperature", "top_k", "top_p", "min_p")
 
 class CategoryChoice:
     """Each parameter is a number for all columns, or a sequence with one for every categorical column (0 / 1.0 / 0.0 leave
-    top_k / top_p / min_p off).  Definitions: `ops.sample_categories`."""
+    top_k / top_p / min_p off; a sequence's temperature, top_p and min_p are rounded to float32).  Definitions:
+    `ops.sample_categories`."""
     __slots__ = _FIELDS
 
     def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-        checks = {"temperature": lambda v: 0.0 <= v < math.inf, "top_k": lambda v: v >= 0 and v == int(v),
+        checks = {"temperature": lambda v: 0.0 <= v <= sys.float_info.max, "top_k": lambda v: 0 <= v < math.inf and v == int(v),
                   "top_p": lambda v: 0.0 <= v <= 1.0, "min_p": lambda v: 0.0 <= v <= 1.0}
         for name, value in zip(_FIELDS, (temperature, top_k, top_p, min_p)):
             each = list(value) if isinstance(value, (list, tuple)) else [value]
@@ -30,6 +32,8 @@ class CategoryChoice:
         out = {}
         for name in _FIELDS:
             v = getattr(self, name)
+            if name == "top_k":                                  # (more than a table has classes, in 32 bits)
+                v = tuple(min(int(k), 2 ** 31 - 1) for k in v) if isinstance(v, tuple) else min(int(v), 2 ** 31 - 1)
             if isinstance(v, tuple):
                 if len(v) != features:
                     raise ValueError(f"CategoryChoice: {len(v)} values of {name} for {features} categorical columns")

@@ -1,5 +1,6 @@
 """What the low-bit layers and the filtered draws check on the host, and what their sources have to hold (no GPU needed)."""
 import ctypes
+import math
 import os
 import re
 
@@ -9,6 +10,7 @@ from torch.autograd import forward_ad
 
 from clavaddpm_amd import ops
 from clavaddpm_amd._lib import ClavaHipError, lib
+from clavaddpm_amd.tab_ddpm import CategoryChoice
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "clavaddpm_amd", "csrc")
 
@@ -111,3 +113,16 @@ def test_a_derivative_that_is_asked_for_is_refused():
         w = some_mx4(0x30000, 0x40000, 3, 3)
         with pytest.raises(ClavaHipError, match="no forward derivative"):
             ops.linear_mx4(some_mx4(0x10000, 0x20000, 4, 3), w, dual)
+
+
+def test_numbers_that_no_parameter_holds():
+    for bad in (dict(top_k=math.inf), dict(top_k=[1, math.inf]), dict(top_k=math.nan), dict(temperature=10 ** 400), dict(temperature=[1.0, 10 ** 400])):
+        with pytest.raises(ValueError, match="CategoryChoice"):
+            CategoryChoice(**bad)
+    cpu = torch.device("cpu")
+    assert CategoryChoice(top_k=[2 ** 40, 3.0, 0]).arguments(3, cpu)["top_k"].tolist() == [2 ** 31 - 1, 3, 0]
+    assert CategoryChoice(top_k=10 ** 30).arguments(3, cpu)["top_k"] == 2 ** 31 - 1
+    for name in ("temperature", "top_p"):
+        with pytest.raises(ClavaHipError, match=name):
+            ops._choice_args(cpu, 1, 1, ((name, 10 ** 400),))
+    assert ops._choice_args(cpu, 1, 1, (("temperature", 10 ** 300),)).temperature == 1e300
