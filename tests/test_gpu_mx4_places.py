@@ -89,3 +89,20 @@ def test_tangents_are_refused_not_lost():
         assert torch.equal(ops.sample_categories(dx, temperature=dt, seed=3), want[1]) and torch.equal(ops.linear_mx4(x, w), want[0])
     with pytest.raises(ClavaHipError, match="backward"):
         ops.sample_categories(x, temperature=t.clone().requires_grad_(), log_prob=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M, N", [(70, 201), (2050, 2101), (5000, 6701)])
+def test_16_bit_results_of_odd_rows_at_odd_places(M, N, dtype):
+    """Rows of the three tiles' results that start at any 2 bytes and end inside a dword: the float32 result's rounding, and
+    nothing beside it."""
+    for K in (300, 512):
+        x, w, bias, _, _ = product_case(M, K, N, M)
+        xq, wq, b = ops.mx4_pack(x.to(DEV)), ops.mx4_pack(w.to(DEV)), bias.to(DEV)
+        want = ops.linear_mx4(xq, wq, b, act="relu").to(dtype)
+        assert torch.equal(ops.linear_mx4(xq, wq, b, act="relu", out_dtype=dtype), want)
+        for start, gap in ((1, 10), (3, 4), (8, 1), (5, 7)):
+            big = torch.full((M + 2, N + gap + start), 9.0, device=DEV, dtype=dtype)
+            ops.linear_mx4(xq, wq, b, act="relu", out=big[1:M + 1, start:start + N])
+            assert torch.equal(big[1:M + 1, start:start + N], want), (K, start)
+            assert (big[0] == 9).all() and (big[M + 1] == 9).all() and (big[:, :start] == 9).all() and (big[:, start + N:] == 9).all(), (K, start)
