@@ -14,9 +14,10 @@
 // block in LDS; wider ones are cut into chunks over many workgroups and joined (wide_*).
 //
 // Each logit is read once up to 2048 classes (wider: three or four times, from the caches mostly), so that memory would need
-// 30 us for 4096 rows of 50 features with 8.1k classes (float32).  They take 115 us, all filters at 20000 rows 768 (145): bound
-// by vector instructions, 254 and 373 a block, three quarters and four fifths of the issue cycles, most of them float64 - a
-// mass takes 20.
+// 35 us for 4096 rows of 50 features with 10 047 classes (float32).  They take 111 us, all filters at 20000 rows 760 (174): bound
+// by vector instructions, 258 and 379 a block, three quarters and four fifths of the issue cycles.  A mass takes 20 (64 classes at
+// once): of the 258 about a third; with the filters it is the passes over the bins, the sort and the sums.  Parameters from
+// tensors: 173 and 1010 us, since every block makes its own out of them.
 #include "elem.h"
 #include "rng.h"
 #include "wave.h"
@@ -906,10 +907,12 @@ template <int DT, int NV, int MODE> __global__ void __launch_bounds__(WAVES * 64
 
 // ------------------------------------------------------------------------------------------- very many classes, in chunks
 // Four launches over chunks of a block (top -> bins -> collect) and over blocks (finish).  Weights are integers, so that the
-// sums over chunks have no order.  64 x 131071 bfloat16 with top-p: 6.7 + 16.2 + 13.0 + 17.0 us; reading it once takes 3.6.  The
-// second is bound by its masses (8.4 million float64 exponentials), the others by the latency of a few dependent loads and
-// workgroup sums; so are all four of 1 x 262144 with top-k (3.0 + 7.6 + 6.4 + 10.0).  Between the launches, for every wide block
-// and in `ws`:
+// sums over chunks have no order.  64 x 131071 bfloat16 with top-p: 7.0 + 16.4 + 13.1 + 16.5 us; reading it once takes 3.6.  Vector
+// instructions issue for 3, 9 and 7 us of the first three (half of the second's are its 8.4 million masses); the rest is the
+// latency of the head, of a few dependent loads and of workgroup sums, and so is nearly all of the last (64 workgroups) and of
+// all four of 1 x 262144 with top-k (3.2 + 7.4 + 6.5 + 9.3).  Where more than WIDE_LIST classes share the edges' bins - logits that
+// are equal, or nearly - one workgroup goes over the whole block: 64 x 131071 equal ones take 2150 us instead of 52, 256 x 50257
+// 1030 instead of 67.  Between the launches, for every wide block and in `ws`:
 constexpr int WT = 256, WIDE_BINS = 256, WIDE_LIST = 4096, WIDE_CHUNKS = 1024;
 struct Wide {
     char* ws;

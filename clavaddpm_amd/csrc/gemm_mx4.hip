@@ -164,8 +164,11 @@ __device__ __forceinline__ void dma4(const void* src, char* dst) {
 // fragment read hit different banks), NS of them in a ring.  Scales have a ring of their own.  S16: 16 bytes of them a row, 512
 // columns, in one copy (rows of whole 16 bytes: K a multiple of 512); else 4 bytes in each.  A copy of scales touches a cache
 // line per row, whatever it takes from it: with 4 bytes the scales took the copies of a 256 x 256 tile from 1.3 to 1.8 us a stage.
-// 16384 x 8192 x 8192 to bfloat16: 518 us, 4.2 PFLOP/s, the matrix cores busy for 48 % of the cycles (at 1.9 GHz); bound by the requests that a
-// CU can have in flight (85 % of them hit L2, which is at a third of its rate), and 11 us a tile of start and result.
+// 16384 x 8192 x 8192 to bfloat16: 1.10 million cycles, 48 % of them with the matrix cores busy: 500 us (4.4 PFLOP/s) to 571 by the
+// clock that a card holds; bound by the requests that a CU can have in flight (85 % of them hit L2, which is at a third of its
+// rate), and 11 us a tile of start and result.  4-bit results of a hidden layer, 20000 x 1024 x 1024: 25 to 28 us (8.1 by its
+// operations, 4.7 by its bytes): a tile has four stages, so that start and result count, and packing the result is vector
+// instructions, 26 000 cycles of a SIMD in all.
 template <int BN, int BM, int WN, int WM, int NS, bool S16, int OUT>
 __global__ void __launch_bounds__(WN * WM * 64) mx4_tile_kernel(Mx4Args g, int tiles_n, int tiles) {
     constexpr int R = BN + BM, NW = WN * WM, Q = R / 8 / NW, STAGE = R * 128;
@@ -421,13 +424,16 @@ template <int OUT> int launch_linear(const Mx4Args& g, hipStream_t st) {
     // a 4-bit result also has the zero codes behind its last column written: its columns go to the whole step
     const int n_cols = OUT == OUT_MX4 ? g.yks * KSTEP : g.N;
     const int tiles_n = (n_cols + 31) / 32;
+    // Few rows (M <= 64) go 16 at a time, which costs most where they are many and the layer is large (us, 16 rows at a time / tiles:
+    // K = N = 1024, M = 17 / 64 / 256: 3.9 / 4.5, 3.9 / 4.6, 5.4 / 4.7; 2048: 5.1 / 5.6, 5.2 / 5.8, 13.2 / 6.0; 4096: 7.7 / 8.0,
+    // 13.1 / 8.2, 44.5 / 9.4; 8192: 20.9 / 13.3, 44.8 / 13.9, 170 / 23.4: from 4096 on the border could be lower).
     // Many rows: the largest tile that still gives every CU two rounds of work (a large tile copies least per product; us for
     // 256 x 256 / 128 x 128 / 64 x 64 tiles, codes to bfloat16: 16384 x 8192 x 8192 540 / 690 / 1083, 20000 x 1024 x 1024
     // 27.7 / 23.3 / 38.8, 4096 x 1024 x 1024 13.9 / 7.7 / 10.3, 1024 x 1024 x 1024 13.0 / 6.4 / 4.7, 256 x 4096 x 4096
     // 30.2 / 13.0 / 8.4).
     auto tiles = [&](int t) { return (long long)((g.M + t - 1) / t) * ((n_cols + t - 1) / t); };
     // The tiles copy scales by dwords.  Those that start between two (a view into a loaded file) are read by bytes, as those of few
-    // rows are: right for any number of rows, but 16 rows at a time.
+    // rows are: right for any number of rows, but 16 at a time (300 x 1024 x 1024 6.9 us instead of 4.9, 20000 rows 248 instead of 25).
     const bool dwords = (((uintptr_t)g.xs | (uintptr_t)g.ws) & 3) == 0;
     if (g.M > 64 && dwords) {
         if (tiles(256) >= 512) return launch_tile<256, 256, 2, 4, 2, OUT>(g, n_cols, st);
@@ -453,7 +459,9 @@ template <int OUT> int launch_linear(const Mx4Args& g, hipStream_t st) {
 
 constexpr int MOST_COLUMNS = 1 << 25;         // 255 rows of codes are inside the 32 bits of a lane's source then
 // Whether floats are packed by a launch of their own: for one tile of rows and few steps of K every workgroup packs them again
-// on the way (1 x 1024 x 1024: 4.6 us, and 5.3 in two launches; 7 x 4099 x 8001: 12.7, and 9.0)
+// on the way.  N hardly counts, since the workgroups pack side by side (us, on the way / first, 16 rows: K = 512, N = 256 and 8192
+// 3.8 / 5.4 and 4.0 / 5.5; 1024: 4.6 / 6.1 and 4.9 / 6.2; 2048: 6.6 / 7.4 and 6.9 / 7.5; 4096: 10.2 / 10.1 and 11.8 / 10.5; one row:
+// 2048: 5.6 / 6.2 and 6.0 / 6.3; 4096: 9.2 / 8.4 and 10.3 / 8.9)
 bool packed_first(int M, int K) { return M > 16 || K > 2048; }
 
 }  // namespace

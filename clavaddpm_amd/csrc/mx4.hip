@@ -2,8 +2,9 @@
 //
 // pack: block of 32 columns -> e = floor(log2(max|v|)) - 2, code = nearest E2M1 of v / 2^e.  Eight columns a lane, so that a
 // block is four neighbouring lanes, its maximum two exchanges and a lane's codes one 4-byte store.
-// unpack: value(code) * 2^e.  Both move each byte once and are bound by that: 20000 x 2000 bfloat16 (101 MB) from memory 21.1 and
-// 24.0 us, 4.8 and 4.2 TB/s; 1999 columns, whose rows start at any 2 bytes, 28 and 28; 4096 x 1024 float32 4.2 and 7.0 us.
+// unpack: value(code) * 2^e.  Both move each byte once and are bound by that: 20000 x 2000 bfloat16 (101 MB) from memory 25.2 and
+// 21.5 us, 4.0 and 4.7 TB/s; 1999 columns, whose rows start at any 2 bytes, 31 and 25; 4096 x 1024 float32 3.8 and 6.9 us (why
+// the second takes longer for the same bytes has not been looked into: its stores fill half a line at a time).
 #include "clava_hip.h"
 #include "mx4.h"
 
@@ -11,7 +12,7 @@ namespace {
 using namespace mx4;
 
 // load8 of a 16-bit type from rows that do not start at 16 bytes: with 16-byte loads at any address 20000 x 1999 bfloat16 took
-// 33 us, this way 28.  A lane loads the aligned 16 bytes that hold its first column, takes the following ones from the next lane
+// 33 us, this way 28 (from memory, in one run).  A lane loads the aligned 16 bytes that hold its first column, takes the following ones from the next lane
 // (`next`: it is the same row's) and shifts them together.  Nothing outside lo .. hi is read: lanes that would, load at any
 // address.  All lanes of a row in the wavefront come here together.
 template <int DT> __device__ __forceinline__ void load8_shifted(const void* src, size_t at, const char* lo, const char* hi, int n, bool next, float* v) {

@@ -251,7 +251,10 @@ int clava_categorical_sampler_set(int mode);
  * temperature 0 takes the first of the order.  A class with z = -inf is never drawn; where some z are +inf, those share the
  * mass equally.  idx[b * m + f] = -1 (log_prob NaN) for a feature without classes, without a z above -inf, or with a NaN in
  * its logits, its u or a parameter, or a negative temperature.  log_prob (optional) [B, m]: log of the drawn class's share of
- * the kept mass.  idx and log_prob may not overlap what is read.  Sums and comparisons are float64 and have a fixed order.
+ * the kept mass.  idx and log_prob may not overlap what is read.  Sums have a fixed order or are whole numbers.  Masses and
+ * comparisons are float64; masses are added in float64, or, for top_p among 65 classes or more and for everything in features of
+ * more than 2048, as whole units of 2^-s of the largest (s = 51 up to 2048 classes, then min(51, 62 - ceil(log2 K))): at most
+ * half a unit a class is lost, K 2^-(s+1) in all of a sum that is at least 1.
  * Each parameter is a number for all blocks, or, where its pointer is not NULL, element [b * rs + f * fs] of a device array.
  * uniforms [b * ld_u + f] in [0, 1), or NULL for the counter-based generator keyed by (seed, row_offset + b, f, step_index).
  * max_k: the largest number of classes of one feature (it picks the kernels and the workspace; any value is safe, a feature of
