@@ -429,7 +429,8 @@ def mx4_pack(x, out=None):
     that holds a NaN or an infinity reads as NaN.  No gradient is defined."""
     rows, cols, ld = _matrix(x, "mx4_pack: x")
     dt = _dt(x, "mx4_pack: x")
-    _no_gradient("mx4_pack has no backward", x)
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _no_gradient("mx4_pack has no backward", x)
     if out is None:
         out = mx4_empty(rows, cols, x.device)
     elif (out.rows, out.cols) != (rows, cols) or out.device != x.device:
@@ -475,6 +476,15 @@ def _parts(t, rows, cols, ld):
         return (t.codes_ptr, 64 * steps, 64 * steps, 1), (t.scales_ptr, 4 * steps, 4 * steps, 1)
     size = t.element_size()
     return ((t.data_ptr(), cols * size, ld * size, rows),)
+
+
+def _ends(p, scales, rows, cols, ld, t):
+    """Where a matrix at `p` begins and ends (scales: None for floats)."""
+    if scales is None:
+        return p, p + ((rows - 1) * ld + cols) * t.element_size()
+    steps = rows * ((cols + 127) // 128)
+    codes_end, scales_end = p + 64 * steps, scales + 4 * steps
+    return (p if p < scales else scales), (codes_end if codes_end > scales_end else scales_end)
 
 
 def _spread(t):
@@ -525,7 +535,8 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
     else:
         M, K, ldx = _matrix(x, "linear_mx4: x")
         x_dt, xp, xs = _dt(x, "linear_mx4: x"), x.data_ptr(), None
-        _no_gradient("linear_mx4 has no backward", x)
+        if x.requires_grad or forward_ad._current_level >= 0:
+            _no_gradient("linear_mx4 has no backward", x)
     if w.cols != K:
         _refuse(f"linear_mx4: x is [{M},{K}] but w is [{N},{w.cols}]")
     if N == 0:
@@ -536,7 +547,8 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
     if bias is not None:
         if bias.dtype is not torch.float32 or bias.shape != (N,) or not bias.is_contiguous() or bias.device != dev:
             _refuse(f"linear_mx4: bias must be contiguous float32 [{N}] on {dev}")
-        _no_gradient("linear_mx4 has no backward", bias)
+        if bias.requires_grad or forward_ad._current_level >= 0:
+            _no_gradient("linear_mx4 has no backward", bias)
         bp = bias.data_ptr()
     if out is None:
         if out_dtype not in _DT:
@@ -552,13 +564,16 @@ def linear_mx4(x, w, bias=None, act=None, out=None, out_dtype=torch.float32):
         if (rows, cols) != (M, N) or out.device != dev:
             _refuse(f"linear_mx4: the result is [{M},{N}] on {dev} but out is [{rows},{cols}] on {out.device}")
         if M:
-            _not_over("linear_mx4", _parts(out, M, N, ldy), x=_parts(x, M, K, ldx), w=_parts(w, N, K, 0),
-                      bias=((bp, 4 * N, 4 * N, 1),) if bp else ())
-    need = 0
-    if x_dt != _MX4:
-        need = _mx4_workspace(M, K, x_dt)
-        if need:
-            ws = torch.empty(need, device=dev, dtype=torch.uint8)
+            # first by the ends of each, which settles nearly every call
+            low, high = _ends(yp, ys, M, N, ldy, out)
+            x_low, x_high = _ends(xp, xs, M, K, ldx, x)
+            w_low, w_high = _ends(w.codes_ptr, w.scales_ptr, N, K, 0, w)
+            if low < x_high and x_low < high or low < w_high and w_low < high or bp is not None and low < bp + 4 * N and bp < high:
+                _not_over("linear_mx4", _parts(out, M, N, ldy), x=_parts(x, M, K, ldx), w=_parts(w, N, K, 0),
+                          bias=((bp, 4 * N, 4 * N, 1),) if bp else ())
+    need = _mx4_workspace(M, K, x_dt) if x_dt != _MX4 else 0
+    if need:
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
     _launch(dev, "clava_linear_mx4_sized", _function("clava_linear_mx4_sized", "pilppppipilpiiiplp"),
             xp, x_dt, ldx, xs, w.codes_ptr, w.scales_ptr, bp, code, yp, y_dt, ldy, ys, M, N, K,
             None if ws is None else ws.data_ptr(), need)
@@ -621,7 +636,7 @@ def sample_categories(logits, uniforms=None, offsets=None, max_classes=None, *, 
     classes whose logits are nearly all equal are slow with top_k or top_p: one workgroup does each (64 rows of 131071: 2.2 ms)."""
     B, sumk, ld = _matrix(logits, "sample_categories: logits")
     dt = _dt(logits, "sample_categories: logits")
-    if log_prob:
+    if log_prob and (logits.requires_grad or isinstance(temperature, torch.Tensor) or forward_ad._current_level >= 0):
         _no_gradient("sample_categories: log_prob has no backward", logits, temperature if isinstance(temperature, torch.Tensor) else None)
     dev = logits.device
     m, op = 1, None
